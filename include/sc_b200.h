@@ -293,6 +293,134 @@ int sc_graph_capture_batch(sc_batch *b, int32_t accumulate, int32_t repeat, sc_g
 int sc_graph_launch(sc_graph *g, void *stream);
 void sc_graph_free(sc_graph *g);
 
+/* --------------------------------------------------------------- serving -- */
+
+/* Operators between the products of a transformer that is served from this
+ * library: keys and values of new tokens into a paged cache (with the rotary
+ * position rotation), attention of one new token per sequence over that
+ * cache, and low-rank adapters of many requests beside a shared projection.
+ * The reference stops at the products (its matrices are transformer weights,
+ * README.md:1-33); these have no counterpart there.
+ *
+ * Element types.  Activations (rows) are fp32, fp16 or bf16 with any strides,
+ * so the feature-major C that sc_spmm writes ((heads * head_dim) x tokens)
+ * is taken as it lies.  All arithmetic, sums and softmax statistics are
+ * fp32; each output is rounded once, to its own type. */
+#define SC_TYPE_F32 0
+#define SC_TYPE_F16 1
+#define SC_TYPE_BF16 2
+
+/* The cache: two pools of `num_pages` pages of `page_size` slots.  Slot s of
+ * page p holds, for each kv head h, head_dim contiguous elements at
+ *   pool + p * stride[0] + h * stride[1] + s * stride[2]   (in elements).
+ * Bases and strides are multiples of 16 bytes, head_dim * element size too;
+ * head_dim <= 256; num_pages * page_size < 2^31 (offsets may pass 32 bits). */
+typedef struct sc_kv_pool {
+  void *k, *v;
+  int64_t num_pages, page_size, kv_heads, head_dim;
+  int64_t k_stride[3], v_stride[3]; /* page, kv head, slot */
+  int64_t type;                     /* SC_TYPE_* of the stored elements */
+} sc_kv_pool;
+
+typedef struct sc_kv_cache sc_kv_cache; /* a pool plus its device status word */
+/* The pool's memory stays the caller's and must outlive the handle. */
+int sc_kv_cache_create(const sc_kv_pool *pool, int32_t device, sc_kv_cache **out);
+void sc_kv_cache_free(sc_kv_cache *c);
+/* Device-side status since the last call (waits for the device, clears it):
+ * 0 = none; 8 = a token's sequence, position or page-table entry was outside
+ * the table or the pool, 9 = a position had no row in the rotation tables.
+ * Such a token is skipped as one with a negative position is; nothing
+ * outside the pool is ever touched. */
+int sc_kv_cache_status(sc_kv_cache *c, int32_t *status);
+
+/* Rows of a (tokens, heads, head_dim) tensor: element strides in that order. */
+typedef struct sc_rows {
+  void *ptr;
+  int64_t stride[3];
+} sc_rows;
+
+typedef struct sc_kv_append_args {
+  int64_t tokens, q_heads;
+  int64_t type;            /* SC_TYPE_* of q, k, v and q_out */
+  sc_rows k, v, q, q_out;  /* q.ptr NULL: no queries; q_out may equal q (same strides) */
+  const int32_t *positions; /* [tokens] place of the token in its sequence; negative: skipped */
+  const int32_t *seq_ids;   /* [tokens] its row of the page table; NULL: token t is of sequence t */
+  const int32_t *page_table; /* [seqs x table_cols], row stride table_stride */
+  int64_t seqs, table_cols, table_stride;
+  const float *cos, *sin;   /* [rope_rows x rotary / 2] fp32, row stride rope_stride; NULL: no rotation */
+  int64_t rope_rows, rope_stride, rotary, interleaved;
+} sc_kv_append_args;
+/* Stores the k and v rows of `tokens` tokens in the cache and rotates k and q
+ * by their positions on the way: with half = rotary / 2, pair i is dims
+ * (i, i + half), or (2i, 2i + 1) when `interleaved`;
+ *   (a, b) -> (a cos - b sin, b cos + a sin),
+ * dims from `rotary` on stay.  A skipped token stores nothing and its q_out
+ * rows become zero.  No two tokens of a call may share a place.  Asynchronous
+ * on `stream`, one kernel launch, no allocation (it may be captured). */
+int sc_kv_append(sc_kv_cache *c, const sc_kv_append_args *a, void *stream);
+
+typedef struct sc_attn sc_attn; /* decode-attention plan: head layout and workspace for a pool */
+/* For up to max_seqs sequences a call; q_heads a multiple of kv_heads (query
+ * heads h*g .. h*g+g-1 read kv head h); scale positive and finite (0: the
+ * usual 1/sqrt(head_dim)); window > 0: only the last `window` keys of a
+ * sequence count (0: all).  Calls with one plan share its workspace: they
+ * must not overlap on the GPU. */
+int sc_attn_create(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, double scale, int64_t window,
+                   sc_attn **out);
+void sc_attn_free(sc_attn *p);
+
+typedef struct sc_attn_args {
+  int64_t seqs;
+  int64_t type;               /* SC_TYPE_* of q and out */
+  sc_rows q, out;             /* (seqs, q_heads, head_dim) */
+  float *lse;                 /* [seqs x q_heads] log of the softmax sums, or NULL */
+  const int32_t *page_table;  /* [seqs x table_cols], row stride table_stride */
+  int64_t table_cols, table_stride;
+  const int32_t *seq_lens;    /* [seqs] keys in the cache, the new token's own included */
+} sc_attn_args;
+/* out = softmax(scale q k^T) v over the keys of each sequence, one query
+ * token per sequence.  A sequence without keys (length <= 0) gives zeros and
+ * lse = -inf.  Asynchronous on `stream`; only kernel launches. */
+int sc_attn_decode(sc_attn *p, const sc_attn_args *a, void *stream);
+/* As sc_kv_cache_status: 8 = a length beyond the page table or a page-table
+ * entry outside the pool; the keys concerned count as absent. */
+int sc_attn_status(sc_attn *p, int32_t *status);
+
+typedef struct sc_adapters sc_adapters; /* a set of low-rank adapters on the device */
+/* Adapter i: down[i] (ranks[i] x in_features, row stride down_ld[i]) and up[i]
+ * (out_features x ranks[i], row stride up_ld[i]), row-major device pointers of
+ * `type`, and a scale.  The weights are copied into the set's own layout
+ * (synchronously, after the work already on `stream`).  Ranks 0 to 256. */
+int sc_adapters_create(int32_t device, int64_t in_features, int64_t out_features, int64_t count,
+                       const int64_t *ranks, int64_t type, const void *const *down, const int64_t *down_ld,
+                       const void *const *up, const int64_t *up_ld, const float *scales, void *stream,
+                       sc_adapters **out);
+void sc_adapters_free(sc_adapters *s);
+/* Scratch bytes that a call with this many tokens needs. */
+int sc_adapters_workspace(const sc_adapters *s, int64_t tokens, int64_t *bytes);
+
+/* A (features, tokens) matrix: element strides in that order, any layout. */
+typedef struct sc_cols {
+  void *ptr;
+  int64_t stride[2];
+} sc_cols;
+
+typedef struct sc_adapters_args {
+  int64_t tokens;
+  int64_t type;        /* SC_TYPE_* of x, base and out */
+  sc_cols x;           /* in_features x tokens, as sc_spmm's B */
+  sc_cols base;        /* out_features x tokens, the shared projection's C; ptr NULL: zeros */
+  sc_cols out;         /* out_features x tokens; may equal base (same strides), never x */
+  const int32_t *ids;  /* [tokens] adapter of each token; negative: none */
+  void *workspace;     /* 16-byte aligned scratch, see sc_adapters_workspace */
+  int64_t workspace_bytes;
+} sc_adapters_args;
+/* out[:, t] = base[:, t] + scale_a up_a (down_a x[:, t]), a = ids[t].
+ * Asynchronous on `stream`; only kernel launches. */
+int sc_adapters_apply(sc_adapters *s, const sc_adapters_args *a, void *stream);
+/* As sc_kv_cache_status: 10 = an id beyond the set (taken as none). */
+int sc_adapters_status(sc_adapters *s, int32_t *status);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,10 @@ this module                                    reference (hosseinal/sparse-compu
 ``SpMMPlan(cf, 1).spmv(x, y)``                 example_cuda/spmv_demo_gpu_utils.h:632-952
 =============================================  =====================================================
 
+Beside the products, ``PagedKVCache``, ``RotaryTable``, ``DecodeAttention`` and
+``LowRankAdapters`` (serving.py) serve a transformer whose weights are such
+matrices; the reference has nothing of that kind.
+
 All numerical work runs in the CUDA kernels of ``libsc_b200.so``; there is no
 CPU fallback.  Importing this module does not need a GPU (the host formats
 and the coarsener are native C++ and run anywhere); creating a plan does.
@@ -62,6 +66,9 @@ EXPORTED_SYMBOLS = (
     "sc_batch_create", "sc_batch_bind", "sc_batch_spmm", "sc_batch_free",
     "sc_spmm_dense_noalloc", "sc_noalloc_status", "sc_plan_status", "sc_batch_status",
     "sc_graph_capture_plan", "sc_graph_capture_batch", "sc_graph_launch", "sc_graph_free",
+    "sc_kv_cache_create", "sc_kv_cache_free", "sc_kv_cache_status", "sc_kv_append",
+    "sc_attn_create", "sc_attn_free", "sc_attn_decode", "sc_attn_status",
+    "sc_adapters_create", "sc_adapters_free", "sc_adapters_workspace", "sc_adapters_apply", "sc_adapters_status",
 )
 
 
@@ -144,6 +151,19 @@ def lib() -> ctypes.CDLL:
         "sc_noalloc_status": ([P(i32)], ctypes.c_int),
         "sc_plan_status": ([vp, P(i32)], ctypes.c_int),
         "sc_batch_status": ([vp, P(i32)], ctypes.c_int),
+        "sc_kv_cache_create": ([vp, i32, P(vp)], ctypes.c_int),
+        "sc_kv_cache_free": ([vp], None),
+        "sc_kv_cache_status": ([vp, P(i32)], ctypes.c_int),
+        "sc_kv_append": ([vp, vp, vp], ctypes.c_int),
+        "sc_attn_create": ([vp, i64, i64, ctypes.c_double, i64, P(vp)], ctypes.c_int),
+        "sc_attn_free": ([vp], None),
+        "sc_attn_decode": ([vp, vp, vp], ctypes.c_int),
+        "sc_attn_status": ([vp, P(i32)], ctypes.c_int),
+        "sc_adapters_create": ([i32, i64, i64, i64, vp, i64, vp, vp, vp, vp, vp, vp, P(vp)], ctypes.c_int),
+        "sc_adapters_free": ([vp], None),
+        "sc_adapters_workspace": ([vp, i64, P(i64)], ctypes.c_int),
+        "sc_adapters_apply": ([vp, vp, vp], ctypes.c_int),
+        "sc_adapters_status": ([vp, P(i32)], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -566,3 +586,6 @@ class Graph:
         if getattr(self, "_h", None) and self._h.value and _lib is not None:
             _lib.sc_graph_free(self._h)
             self._h = ctypes.c_void_p()
+
+
+from .serving import DecodeAttention, LowRankAdapters, PagedKVCache, RotaryTable  # noqa: E402,F401
