@@ -1,4 +1,4 @@
-// Cache append with rotary rotation, and decode attention over a paged cache.
+// Cache append with the rotary rotation.
 #include <cmath>
 #include <memory>
 
@@ -8,7 +8,7 @@ using namespace sc::serve;
 
 namespace {
 
-constexpr int64_t kMaxHeadDim = 256;
+constexpr int64_t kMaxHeadDim = 256;  // the widest tile of the attention kernel
 
 // --------------------------------------------------------------- append ----
 
@@ -95,70 +95,6 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
   }
 }
 
-// --------------------------------------------------------------- attend ----
-
-struct AttnParams {
-  sc_attn_args a;
-  sc_kv_pool pool;
-  int q_heads, group;
-  float scale;
-  int64_t window;
-  int *status;
-};
-
-// One block per (sequence, query head): each warp walks its share of the keys
-// with a running maximum and sum, the four warps are joined at the end.
-template <class T, class C>
-__global__ void __launch_bounds__(128) attend_kernel(const AttnParams p) {
-  __shared__ float sq[kMaxHeadDim], sm[4], sl[4], so[4][kMaxHeadDim];
-  const int seq = blockIdx.x, head = blockIdx.y, d = (int)p.pool.head_dim, ps = (int)p.pool.page_size;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const T *q = static_cast<const T *>(p.a.q.ptr) + seq * p.a.q.stride[0] + head * p.a.q.stride[1];
-  for (int i = threadIdx.x; i < d; i += 128) sq[i] = to_f32(q[i * p.a.q.stride[2]]) * p.scale;
-  __syncthreads();
-  int64_t len = p.a.seq_lens[seq];
-  if (len > p.a.table_cols * ps) {
-    set_status(p.status, 8);
-    len = p.a.table_cols * ps;
-  }
-  const int64_t first = p.window && len > p.window ? len - p.window : 0;
-  const int kvh = head / p.group;
-  float m = -INFINITY, l = 0.f, o[kMaxHeadDim / 32] = {};
-  for (int64_t j = first + warp; j < len; j += 4) {
-    const int page = p.a.page_table[seq * p.a.table_stride + j / ps];
-    if (page < 0 || page >= p.pool.num_pages) {
-      if (lane == 0) set_status(p.status, 8);
-      continue;
-    }
-    const C *k = static_cast<const C *>(p.pool.k) + page * p.pool.k_stride[0] + kvh * p.pool.k_stride[1] +
-                 (j % ps) * p.pool.k_stride[2];
-    const C *v = static_cast<const C *>(p.pool.v) + page * p.pool.v_stride[0] + kvh * p.pool.v_stride[1] +
-                 (j % ps) * p.pool.v_stride[2];
-    float z = 0.f;
-    for (int i = lane; i < d; i += 32) z += sq[i] * to_f32(k[i]);
-    for (int s = 16; s; s >>= 1) z += __shfl_xor_sync(~0u, z, s);
-    const float top = fmaxf(m, z), ref = top == -INFINITY ? 0.f : top;
-    const float shrink = expf(m - ref), w = expf(z - ref);
-    l = l * shrink + w;
-    m = top;
-    for (int i = 0; i < kMaxHeadDim / 32; ++i)
-      if (lane + 32 * i < d) o[i] = o[i] * shrink + w * to_f32(v[lane + 32 * i]);
-  }
-  if (lane == 0) sm[warp] = m, sl[warp] = l;
-  for (int i = 0; i < kMaxHeadDim / 32; ++i) so[warp][lane + 32 * i] = o[i];
-  __syncthreads();
-  const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), ref = top == -INFINITY ? 0.f : top;
-  float total = 0.f;
-  for (int w = 0; w < 4; ++w) total += sl[w] * expf(sm[w] - ref);
-  T *out = static_cast<T *>(p.a.out.ptr) + seq * p.a.out.stride[0] + head * p.a.out.stride[1];
-  for (int i = threadIdx.x; i < d; i += 128) {
-    float y = 0.f;
-    for (int w = 0; w < 4; ++w) y += so[w][i] * expf(sm[w] - ref);
-    out[i * p.a.out.stride[2]] = from_f32<T>(total == 0.f ? 0.f : y / total);
-  }
-  if (p.a.lse && threadIdx.x == 0) p.a.lse[(int64_t)seq * p.q_heads + head] = ref + logf(total);
-}
-
 template <class F>
 void with_types(int64_t rows, int64_t cache, F f) {
   auto inner = [&](auto t) {
@@ -195,20 +131,6 @@ void check_pool(const sc_kv_pool &p) {
 }
 
 }  // namespace
-
-struct sc_kv_cache {
-  sc_kv_pool pool;
-  int device = 0;
-  DeviceBlock status;
-};
-
-struct sc_attn {
-  sc_kv_pool pool;
-  int device = 0;
-  int64_t q_heads = 0, max_seqs = 0, window = 0;
-  float scale = 0.f;
-  DeviceBlock status;
-};
 
 extern "C" {
 
@@ -260,59 +182,6 @@ int sc_kv_append(sc_kv_cache *c, const sc_kv_append_args *a, void *stream) {
         <<<(unsigned)((n + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
   });
   cuda_check(cudaGetLastError(), "launch cache append");
-  SC_SERVE_END
-}
-
-int sc_attn_create(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, double scale, int64_t window,
-                   sc_attn **out) {
-  SC_SERVE_BEGIN
-  require(cache && out, SC_ERR_ARG, "null argument");
-  *out = nullptr;
-  require(q_heads > 0 && q_heads % cache->pool.kv_heads == 0 && q_heads <= 65535, SC_ERR_ARG,
-          "q_heads must be a positive multiple of kv_heads");
-  require(max_seqs > 0 && max_seqs <= (1 << 20), SC_ERR_ARG, "max_seqs must be 1 to 2^20");
-  require(std::isfinite(scale) && scale >= 0, SC_ERR_ARG, "scale must be positive and finite");
-  require(window >= 0, SC_ERR_ARG, "negative window");
-  std::unique_ptr<sc_attn> p(new sc_attn);
-  p->pool = cache->pool;
-  p->device = cache->device;
-  p->q_heads = q_heads;
-  p->max_seqs = max_seqs;
-  p->window = window;
-  p->scale = (float)(scale > 0 ? scale : 1.0 / std::sqrt((double)cache->pool.head_dim));
-  DeviceGuard dg(p->device);
-  p->status.alloc(p->device, 256, "allocate status word");
-  cuda_check(cudaMemset(p->status.p, 0, 256), "clear status word");
-  *out = p.release();
-  SC_SERVE_END
-}
-
-void sc_attn_free(sc_attn *p) { delete p; }
-
-int sc_attn_status(sc_attn *p, int32_t *status) {
-  SC_SERVE_BEGIN
-  require(p && status, SC_ERR_ARG, "null argument");
-  *status = take_status(p->device, static_cast<int *>(p->status.p));
-  SC_SERVE_END
-}
-
-int sc_attn_decode(sc_attn *p, const sc_attn_args *a, void *stream) {
-  SC_SERVE_BEGIN
-  require(p && a, SC_ERR_ARG, "null argument");
-  require(a->seqs >= 0 && a->seqs <= p->max_seqs, SC_ERR_ARG, "more sequences than the plan's max_seqs");
-  if (a->seqs == 0) return SC_OK;
-  require(type_ok(a->type), SC_ERR_ARG, "unknown element type");
-  require(a->q.ptr && a->out.ptr && a->page_table && a->seq_lens, SC_ERR_ARG,
-          "null q, out, page table or lengths");
-  require(a->table_cols >= 0 && a->table_stride >= 0, SC_ERR_ARG, "bad page table sizes");
-  AttnParams k{*a, p->pool, (int)p->q_heads, (int)(p->q_heads / p->pool.kv_heads), p->scale, p->window,
-               static_cast<int *>(p->status.p)};
-  DeviceGuard dg(p->device);
-  with_types(a->type, p->pool.type, [&](auto t, auto e) {
-    attend_kernel<decltype(t), decltype(e)>
-        <<<dim3((unsigned)a->seqs, (unsigned)p->q_heads), 128, 0, static_cast<cudaStream_t>(stream)>>>(k);
-  });
-  cuda_check(cudaGetLastError(), "launch decode attention");
   SC_SERVE_END
 }
 

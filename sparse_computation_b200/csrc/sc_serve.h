@@ -72,6 +72,12 @@ inline bool type_ok(int64_t t) { return t == SC_TYPE_F32 || t == SC_TYPE_F16 || 
 }  // namespace serve
 }  // namespace sc
 
+struct sc_kv_cache {
+  sc_kv_pool pool;
+  int device = 0;
+  sc::serve::DeviceBlock status;
+};
+
 #define SC_SERVE_BEGIN try {
 #define SC_SERVE_END                        \
   }                                         \
