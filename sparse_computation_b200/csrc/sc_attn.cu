@@ -13,23 +13,32 @@ namespace {
 // One instantiation of the kernel and what its launch needs.
 struct Variant {
   void (*kernel)(Params);
-  int smem, tile, record, per_sm;
+  int warps, smem, keys, piece;
 };
 
+// As many warps as registers (16, or 8 from head_dim 129 on) and shared
+// memory allow: each has its K and V slots and its query tile.
 template <int MODE, int DP>
-Variant variant() {
+Variant variant(int q_rows, int smem_limit) {
   using C = Cfg<MODE, DP>;
-  Variant v{attend_kernel<MODE, DP>, C::smem, C::tile, C::record, 0};
-  cuda_check(cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem),
+  const int per_warp = C::kv + C::q_row * q_rows;
+  Variant v{attend_kernel<MODE, DP>, 0, 0, C::keys, C::piece};
+  cudaFuncAttributes attr;
+  cuda_check(cudaFuncGetAttributes(&attr, v.kernel), "kernel attributes");
+  v.warps = std::min(C::max_warps, (smem_limit - (int)attr.sharedSizeBytes) / per_warp);
+  v.smem = v.warps * per_warp;
+  require(v.warps > 0, SC_ERR_CUDA, "the attention kernel does not fit this GPU");
+  cuda_check(cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  smem_limit - (int)attr.sharedSizeBytes),
              "set shared memory size");
-  cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v.per_sm, v.kernel, kThreads, v.smem), "occupancy");
-  require(v.per_sm > 0, SC_ERR_CUDA, "the attention kernel does not fit this GPU");
   return v;
 }
 
 template <int MODE>
-Variant variant_for(int64_t head_dim) {
-  return head_dim <= 64 ? variant<MODE, 64>() : head_dim <= 128 ? variant<MODE, 128>() : variant<MODE, 256>();
+Variant variant_for(int64_t head_dim, int q_rows, int smem_limit) {
+  return head_dim <= 64    ? variant<MODE, 64>(q_rows, smem_limit)
+         : head_dim <= 128 ? variant<MODE, 128>(q_rows, smem_limit)
+                           : variant<MODE, 256>(q_rows, smem_limit);
 }
 
 }  // namespace
@@ -39,11 +48,12 @@ struct sc_attn {
   int device = 0;
   int64_t q_heads = 0, max_seqs = 0, window = 0;
   float scale = 0.f;
-  int qtiles = 0, sms = 0, min_tiles = 1;
+  int qtiles = 0, q_rows = 0, sms = 0;
+  uint32_t page_mul = 0, page_shift = 0;
   Variant same, other;  // q of the cache's type; q of another type
-  DeviceBlock mem;      // status | arrivals | partial records
+  DeviceBlock mem;      // status | arrivals | pieces | records
   int *status = nullptr, *arrivals = nullptr;
-  float *partials = nullptr;
+  float *heads = nullptr, *records = nullptr;
 };
 
 extern "C" {
@@ -69,27 +79,36 @@ int sc_attn_create(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, 
   p->qtiles = (int)((q_heads / pool.kv_heads + kQT - 1) / kQT);
   const int64_t segments = max_seqs * pool.kv_heads * p->qtiles;
   require(segments < INT32_MAX, SC_ERR_UNSUPPORTED, "max_seqs times heads reaches 2^31");
+  p->q_rows = (int)std::min<int64_t>(q_heads / pool.kv_heads, kQT);
+  // key / page_size for keys below 2^31: multiply by 2^(31 + bits) / page_size, rounded up
+  for (int bits = 1; pool.page_size > 1; ++bits)
+    if (((int64_t)1 << bits) >= pool.page_size) {
+      p->page_mul = (uint32_t)((((uint64_t)1 << (31 + bits)) + pool.page_size - 1) / pool.page_size);
+      p->page_shift = bits - 1;
+      break;
+    }
   DeviceGuard dg(p->device);
+  int limit = 0;
   cuda_check(cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, p->device), "device attribute");
+  cuda_check(cudaDeviceGetAttribute(&limit, cudaDevAttrMaxSharedMemoryPerBlockOptin, p->device), "device attribute");
   if (pool.type == SC_TYPE_F32) {
-    p->same = p->other = variant_for<kTF32>(pool.head_dim);
+    p->same = p->other = variant_for<kTF32>(pool.head_dim, p->q_rows, limit);
   } else if (pool.type == SC_TYPE_F16) {
-    p->same = variant_for<kF16>(pool.head_dim);
-    p->other = variant_for<kF16Wide>(pool.head_dim);
+    p->same = variant_for<kF16>(pool.head_dim, p->q_rows, limit);
+    p->other = variant_for<kF16Wide>(pool.head_dim, p->q_rows, limit);
   } else {
-    p->same = variant_for<kBF16>(pool.head_dim);
-    p->other = variant_for<kBF16Wide>(pool.head_dim);
+    p->same = variant_for<kBF16>(pool.head_dim, p->q_rows, limit);
+    p->other = variant_for<kBF16Wide>(pool.head_dim, p->q_rows, limit);
   }
-  const size_t blocks = (size_t)std::max(p->same.per_sm, p->other.per_sm) * p->sms;
-  require(blocks * kQT * 4 <= (size_t)std::min(p->same.smem, p->other.smem), SC_ERR_UNSUPPORTED,
-          "more blocks than the join has room for");
-  const size_t words = 64 + ((size_t)segments + 63) / 64 * 64;
-  p->mem.alloc(p->device, words * 4 + blocks * 2 * p->same.record * 4, "allocate attention workspace");
+  const size_t words = 64 + ((size_t)segments + 63) / 64 * 64, piece = (size_t)p->same.piece;
+  const size_t heads = (size_t)p->sms * std::max(p->same.warps, p->other.warps) * piece;
+  p->mem.alloc(p->device, (words + heads + (size_t)p->sms * 2 * piece) * 4, "allocate attention workspace");
   cuda_check(cudaMemset(p->mem.p, 0, words * 4), "clear attention workspace");
   cuda_check(cudaDeviceSynchronize(), "device synchronize");
   p->status = static_cast<int *>(p->mem.p);
   p->arrivals = p->status + 64;
-  p->partials = reinterpret_cast<float *>(p->status + words);
+  p->heads = reinterpret_cast<float *>(p->status + words);
+  p->records = p->heads + heads;
   *out = p.release();
   SC_SERVE_END
 }
@@ -112,16 +131,20 @@ int sc_attn_decode(sc_attn *p, const sc_attn_args *a, void *stream) {
   require(a->q.ptr && a->out.ptr && a->page_table && a->seq_lens, SC_ERR_ARG,
           "null q, out, page table or lengths");
   require(a->table_cols >= 0 && a->table_stride >= 0, SC_ERR_ARG, "bad page table sizes");
+  const int64_t e = type_bytes(a->type);
+  const int q_vec = a->q.stride[2] == 1 && a->q.stride[1] * e % 16 == 0 && a->q.stride[0] * e % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(a->q.ptr) % 16 == 0 && p->pool.head_dim % 8 == 0;
   const Variant &v = a->type == p->pool.type ? p->same : p->other;
-  Params k{*a,           p->pool,    (int)p->q_heads, (int)(p->q_heads / p->pool.kv_heads), p->qtiles, p->min_tiles,
-           (float)(p->scale * 1.4426950408889634), p->window, p->status, p->arrivals, p->partials};
-  // the most tiles that these lengths can have; the true number is known on the device only
+  Params k{*a, p->pool, (int)p->q_heads, (int)(p->q_heads / p->pool.kv_heads), p->qtiles, p->q_rows, v.warps,
+           p->page_mul, p->page_shift, q_vec, (float)(p->scale * 1.4426950408889634), p->window, p->status, p->arrivals,
+           p->heads, p->records};
+  // the most steps that these lengths can have; the true number is known on the device only
   int64_t keys = std::min<int64_t>(a->table_cols, INT32_MAX / p->pool.page_size) * p->pool.page_size;
   if (p->window) keys = std::min(keys, p->window + 15);
-  const int64_t tiles = std::max<int64_t>(1, (keys + v.tile - 1) / v.tile) * a->seqs * p->pool.kv_heads * p->qtiles;
-  const int64_t blocks = std::min<int64_t>(tiles, (int64_t)v.per_sm * p->sms);
+  const int64_t steps = std::max<int64_t>(1, (keys + v.keys - 1) / v.keys) * a->seqs * p->pool.kv_heads * p->qtiles;
+  const int64_t blocks = std::min<int64_t>((steps + v.warps - 1) / v.warps, p->sms);
   DeviceGuard dg(p->device);
-  v.kernel<<<(unsigned)blocks, kThreads, v.smem, static_cast<cudaStream_t>(stream)>>>(k);
+  v.kernel<<<(unsigned)blocks, v.warps * 32, v.smem, static_cast<cudaStream_t>(stream)>>>(k);
   cuda_check(cudaGetLastError(), "launch decode attention");
   SC_SERVE_END
 }

@@ -7,7 +7,7 @@
 // the bound is the memory read, and everything here serves to keep enough
 // reads in flight.
 //
-// Matrix instructions.  A warp takes 16 (or 8) keys at a time and computes
+// Matrix instructions.  A warp takes kKeys keys at a time and computes
 // S = Q K^T and O += P V with mma.sync, the 8 query heads of a tile in rows
 // 0-7.  Rows 8-15 carry what a single 16-bit or TF32 operand loses: Q and P
 // are split into a head (rows 0-7) and a tail (rows 8-15), and the two halves
@@ -18,16 +18,22 @@
 // takes whole 16-byte pieces: of K, piece t + 4j of key g (g = lane / 4,
 // t = lane % 4) is a B fragment of 2 k-steps; of V, piece g + 8j of keys
 // 2t, 2t+1 (+8) holds one column of O per element.  A lane therefore only
-// ever reads back what it copied itself: its cp.async ring in shared memory
-// needs no barrier, only its own wait_group.
+// ever reads back what it copied itself: its cp.async slots in shared memory
+// need no barrier, only its own wait_group.  Each warp has one slot for K and
+// one for V; the next K is asked for as soon as the scores are done, the next
+// V after the product with P.  With 16 warps a SM and 8 KB a warp step that
+// keeps 64-128 KB in flight, more than latency times bandwidth asks for.
 //
-// Work.  All (sequence, kv head, query tile) segments are cut into tiles of
-// kTile keys and laid end to end; every block takes one equal, contiguous run
-// of tiles, found by a scan over the sequence lengths on the device (the host
-// never sees them).  A segment that one block covers is written directly;
-// otherwise its blocks leave partial (m, l, O) records in the workspace and
-// the last one to arrive adds them up in block order, so results do not
-// depend on the order of arrival.
+// Work.  All (sequence, kv head, query tile) segments are cut into steps of
+// kKeys keys and laid end to end.  Every block takes one equal, contiguous
+// run of steps, found by a scan over the sequence lengths on the device (the
+// host never sees them), and every warp an equal share of its block's run.
+// Warps do not wait for one another until all are done: a segment that one
+// warp covers is written directly, the others leave pieces (m, l, O) that the
+// block adds up at its end.  A segment that passes the end of a block's run
+// goes into a record in the workspace, and the last of its blocks to arrive
+// adds the records up.  Pieces and records are added in the order of the
+// keys, so results do not depend on the order of arrival.
 #pragma once
 
 #include "sc_serve.h"
@@ -37,37 +43,41 @@ namespace attn {
 
 using serve::to_f32;
 
-constexpr int kWarps = 4, kThreads = kWarps * 32, kQT = 8;
+constexpr int kQT = 8, kMaxWarps = 16;
 
 enum Mode { kTF32, kBF16, kBF16Wide, kF16, kF16Wide };
 
 struct Params {
   sc_attn_args a;
   sc_kv_pool pool;
-  int q_heads, group, qtiles, min_tiles;
-  float scale_log2;  // scale * log2(e)
+  int q_heads, group, qtiles, q_rows;  // q_rows: rows of a query tile, min(group, kQT)
+  int min_run;                         // fewest steps of a block
+  uint32_t page_mul, page_shift;       // key / page_size = umulhi(key, mul) >> shift (mul 0: page_size 1)
+  int q_vec;                           // query rows are contiguous and 16-byte aligned
+  float scale_log2;                    // scale * log2(e)
   int64_t window;
   int *status;
-  int *arrivals;    // [seqs * kv_heads * qtiles], zero between calls
-  float *partials;  // [blocks][2][kQT * (DP + 2)]
+  int *arrivals;   // [seqs * kv_heads * qtiles], zero between calls
+  float *heads;    // [blocks][warps] pieces whose warp went on after them
+  float *records;  // [blocks][2]
 };
 
 template <int MODE, int DP>
 struct Cfg {
   static constexpr bool f32 = MODE == kTF32;
   static constexpr int es = f32 ? 4 : 2, epc = 16 / es;  // bytes per element, elements per 16-byte piece
-  static constexpr int NT = f32 && DP > 64 ? 1 : 2;      // 8-key columns of S per warp step
+  // 8-key columns of S per step: 8 KB of K and V (16 KB from head_dim 129 on)
+  static constexpr int NT = f32 ? (DP > 64 ? 1 : 2) : (DP > 64 ? 2 : 4);
   static constexpr int KJ = DP / (4 * epc), VJ = (DP + 8 * epc - 1) / (8 * epc);
-  static constexpr int slots = NT * KJ + 2 * NT * VJ, stage = slots * 512;
-  static constexpr int NST = stage <= 4096 ? 4 : stage <= 8192 ? 3 : 2;
+  static constexpr int k_slots = NT * KJ, v_slots = 2 * NT * VJ, kv = (k_slots + v_slots) * 512;
   static constexpr int parts = MODE == kBF16Wide ? 3 : MODE == kBF16 || MODE == kF16 ? 1 : 2;  // of Q
-  static constexpr int keys = NT * 8, tile = keys * kWarps;
-  static constexpr int q_bytes = KJ * parts * 512;
-  static constexpr int ring = kWarps * NST * stage;
-  static constexpr int smem = ring + q_bytes;
-  static constexpr int o_row = DP + 4;
-  static constexpr int record = kQT * (DP + 2);  // floats of a partial record
-  static_assert(NST * stage >= kQT * o_row * 4, "a warp's ring holds its O for the join");
+  static constexpr int keys = NT * 8;
+  static constexpr int sub = keys < 16 ? keys : 16;  // keys that lie in one page when page_size is a multiple of 16
+  static constexpr int q_row = KJ * parts * 64;      // bytes of one query row in fragment order
+  static constexpr int max_warps = DP > 128 ? 8 : kMaxWarps;
+  static constexpr int o_row = DP + 4;               // floats; the pad spreads rows over the banks
+  static constexpr int piece = kQT * o_row + 2 * kQT;  // O | m | l
+  static_assert(kv >= piece * 4, "a warp's slots hold its last piece");
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -127,11 +137,6 @@ __device__ __forceinline__ uint32_t pack2(float &a, float &b) {
   }
 }
 
-__device__ __forceinline__ float load_row(const void *p, int64_t type, int64_t i) {
-  if (type == SC_TYPE_F32) return static_cast<const float *>(p)[i];
-  if (type == SC_TYPE_F16) return to_f32(static_cast<const __half *>(p)[i]);
-  return to_f32(static_cast<const __nv_bfloat16 *>(p)[i]);
-}
 __device__ __forceinline__ void store_row(void *p, int64_t type, int64_t i, float x) {
   if (type == SC_TYPE_F32)
     static_cast<float *>(p)[i] = x;
@@ -141,13 +146,13 @@ __device__ __forceinline__ void store_row(void *p, int64_t type, int64_t i, floa
     static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
 }
 
-// Keys [first, len) of a sequence; the tiles start at `start`, first rounded
-// down to a multiple of 16 so that no warp step straddles a page whose size is one.
+// Keys [first, len) of a sequence; steps start at `start`, first rounded down
+// to a multiple of 16 so that no step straddles a page whose size is one.
 struct Span {
-  int first, len, start, tiles;
+  int first, len, start, steps;
 };
 
-template <int TILE>
+template <int KEYS>
 __device__ __forceinline__ Span span_of(const Params &p, int64_t s) {
   Span r;
   r.len = max(p.a.seq_lens[s], 0);
@@ -158,52 +163,200 @@ __device__ __forceinline__ Span span_of(const Params &p, int64_t s) {
   }
   r.first = p.window && r.len > p.window ? r.len - (int)p.window : 0;
   r.start = r.first & ~15;
-  r.tiles = (r.len - r.start) / TILE + ((r.len - r.start) % TILE != 0);
+  r.steps = (r.len - r.start) / KEYS + ((r.len - r.start) % KEYS != 0);
   return r;
 }
 
+__device__ __forceinline__ int page_of(const Params &p, int key) {
+  return p.page_mul ? (int)(__umulhi((uint32_t)key, p.page_mul) >> p.page_shift) : key;
+}
+
+// Four neighbouring outputs from dim d on of one head.
+__device__ __forceinline__ void store4(const Params &p, int64_t seq, int head, int d, float4 y) {
+  const int64_t st = p.a.out.stride[2];
+  const int64_t i = seq * p.a.out.stride[0] + head * p.a.out.stride[1] + d * st;
+  const float v[4] = {y.x, y.y, y.z, y.w};
+  for (int e = 0; e < 4; ++e) store_row(p.a.out.ptr, p.a.type, i + e * st, v[e]);
+}
+
+__device__ __forceinline__ float lse_of(float ref, float sum) { return (ref + log2f(sum)) * 0.69314718055994531f; }
+
+// A boundary between two blocks' runs: the place that an equal cut gives,
+// moved to an end of its segment when that is near, which saves a join.
+struct Cut {
+  int64_t at, seq, seq_begin, seg_begin, seg_end;
+};
+
+__device__ __forceinline__ int64_t snapped(int64_t b, int64_t x, int64_t y, int64_t near) {
+  const int64_t lo = b - x, hi = y - b;
+  return lo <= near && lo <= hi ? x : hi <= near ? y : b;
+}
+
+// N neighbouring elements of a query row from dim d on, as floats; zeros from head_dim on.
+template <int N, class T>
+__device__ __forceinline__ void load_dims(const T *q, const Params &p, int d, float (&x)[N]) {
+  const int D = (int)p.pool.head_dim;
+  if (p.q_vec) {  // contiguous and aligned: head_dim is a multiple of N then
+    if (d >= D) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] = 0.f;
+    } else {
+      constexpr int words = N * (int)sizeof(T) / 8;
+      uint2 w[words];
+#pragma unroll
+      for (int i = 0; i < words; ++i) w[i] = reinterpret_cast<const uint2 *>(q + d)[i];
+      const T *v = reinterpret_cast<const T *>(w);
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] = to_f32(v[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = d + e < D ? to_f32(q[(d + e) * p.a.q.stride[2]]) : 0.f;
+  }
+}
+
+// Puts a lane's share of query row q (pieces t, t + 4, ...) into fragment
+// order, split into parts.  For fp16 parts a row is scaled by a power of two
+// to below 2, so that no part overflows and the tails stay above fp16's
+// smallest values; returns that factor.  The four lanes of a row call it together.
+template <int MODE, int DP, class T>
+__device__ __forceinline__ float fill_q(const T *q, const Params &p, int t, uint32_t sq, int q_step, uint32_t group) {
+  using C = Cfg<MODE, DP>;
+  float x[C::KJ][C::epc], up = 1.f;
+#pragma unroll
+  for (int j = 0; j < C::KJ; ++j) load_dims<C::epc>(q, p, (t + 4 * j) * C::epc, x[j]);
+  if (MODE == kF16Wide) {
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < C::KJ; ++j)
+#pragma unroll
+      for (int e = 0; e < C::epc; ++e) top = fmaxf(top, fabsf(x[j][e]));
+    top = fmaxf(top, __shfl_xor_sync(group, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(group, top, 2));
+    const int e = (int)(__float_as_uint(top) >> 23) - 127;  // floor(log2(top)) of a normal number
+    if (e > -120 && e < 127) up = __uint_as_float((uint32_t)(e + 127) << 23);
+  }
+#pragma unroll
+  for (int j = 0; j < C::KJ; ++j) {
+    if (MODE == kF16Wide)
+#pragma unroll
+      for (int e = 0; e < C::epc; ++e) x[j][e] *= 1.f / up;
+#pragma unroll
+    for (int part = 0; part < C::parts; ++part) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (C::f32)
+          w[e] = part ? tf32_tail(x[j][e]) : tf32_head(x[j][e]);
+        else
+          w[e] = pack2<MODE>(x[j][(2 * e) % C::epc], x[j][(2 * e + 1) % C::epc]);
+      }
+      asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(sq + (j * C::parts + part) * q_step), "r"(w[0]),
+                   "r"(w[1]), "r"(w[2]), "r"(w[3])
+                   : "memory");
+    }
+  }
+  return up;
+}
+
+// Adds up row r of pieces (m, l, O); a lane takes dims 4 lane, 4 lane + 128, ...
+// List gives the first piece's number, the next one's (-1: none) and a piece's place.
+template <int DP, class List>
+__device__ __forceinline__ void add_up(const List &list, int r, float4 (&y)[(DP + 127) / 128], float &ref, float &sum) {
+  constexpr int ND = (DP + 127) / 128, o_row = DP + 4;
+  const int lane = threadIdx.x % 32;
+  float top = -INFINITY;
+  for (int i = list.first(); i >= 0; i = list.next(i)) top = fmaxf(top, list.load(list.at(i) + kQT * o_row + r));
+  ref = top == -INFINITY ? 0.f : top;
+  sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < ND; ++k) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = list.first(); i >= 0; i = list.next(i)) {
+    const float *q = list.at(i);
+    const float f = ex2(list.load(q + kQT * o_row + r) - ref);
+    sum += f * list.load(q + kQT * o_row + kQT + r);
+#pragma unroll
+    for (int k = 0; k < ND; ++k) {
+      const int d = 4 * lane + 128 * k;
+      if (d < DP) {
+        const float4 v = list.load(reinterpret_cast<const float4 *>(q + r * o_row + d));
+        y[k].x += f * v.x, y[k].y += f * v.y, y[k].z += f * v.z, y[k].w += f * v.w;
+      }
+    }
+  }
+}
+
+// The pieces of one segment in a block: even numbers in the workspace, odd ones in the warps' slots.
+struct PieceList {
+  uint32_t members;
+  const float *heads;  // of the block
+  const uint8_t *smem;
+  int piece, warp_bytes;
+  template <class T>
+  __device__ T load(const T *q) const { return *q; }  // shared or global memory, of this block's own writing
+  __device__ int first() const { return __ffs(members) - 1; }
+  __device__ int next(int i) const { return i == 31 ? -1 : __ffs(members & (~0u << (i + 1))) - 1; }
+  __device__ const float *at(int i) const {
+    return i % 2 ? reinterpret_cast<const float *>(smem + (i / 2) * warp_bytes) : heads + (i / 2) * piece;
+  }
+};
+
+// The records of a segment: of the block where it begins, then of those that it runs through.
+struct RecordList {
+  const float *records;
+  int piece, from, to;
+  template <class T>
+  __device__ T load(const T *q) const { return __ldcg(q); }  // written by other blocks
+  __device__ int first() const { return from; }
+  __device__ int next(int b) const { return b < to ? b + 1 : -1; }
+  __device__ const float *at(int b) const { return records + ((int64_t)b * 2 + (b == from)) * piece; }
+};
+
 template <int MODE, int DP>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const Params p) {
+__global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kernel(const Params p) {
   using C = Cfg<MODE, DP>;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t s_scan[kWarps];
-  __shared__ int64_t s_found[2];
-  __shared__ float s_scale[kQT], s_m[kWarps][kQT], s_l[kWarps][kQT], s_top[kQT], s_sum[kQT];
+  __shared__ int64_t s_scan[kMaxWarps];
+  __shared__ Cut s_cut[2];
+  __shared__ int64_t s_seg[2 * kMaxWarps], s_end[2 * kMaxWarps], s_seq[2 * kMaxWarps], s_unit[2 * kMaxWarps];
+  __shared__ uint32_t s_masks[2];
   __shared__ int s_last;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
-  const int D = (int)p.pool.head_dim, H = (int)p.pool.kv_heads;
+  const int W = blockDim.x / 32, D = (int)p.pool.head_dim;
   const int ps = (int)p.pool.page_size;
-  const int64_t units = (int64_t)H * p.qtiles;  // segments of a sequence
+  const int64_t units = p.pool.kv_heads * p.qtiles;  // segments of a sequence
 
-  // ---- this block's run of tiles
+  // ---- this block's run of steps
   int64_t mine = 0;
-  for (int64_t s = tid; s < p.a.seqs; s += kThreads) mine += span_of<C::tile>(p, s).tiles;
+  for (int64_t s = tid; s < p.a.seqs; s += blockDim.x) mine += span_of<C::keys>(p, s).steps;
   for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(~0u, mine, d);
   if (lane == 0) s_scan[warp] = mine;
   __syncthreads();
   int64_t total = 0;
-  for (int w = 0; w < kWarps; ++w) total += s_scan[w];
+  for (int w = 0; w < W; ++w) total += s_scan[w];
   total *= units;
   int64_t per = (total + gridDim.x - 1) / gridDim.x;
-  if (per < p.min_tiles) per = p.min_tiles;
-  const int64_t begin = per * blockIdx.x, end = begin + per < total ? begin + per : total;
+  if (per < p.min_run) per = p.min_run;
+  const int64_t near = max(per / 8, min(per, (int64_t)W) / 2);
 
   // sequences without keys
   for (int64_t s = blockIdx.x; s < p.a.seqs; s += gridDim.x)
-    if (span_of<C::tile>(p, s).tiles == 0) {
-      for (int i = tid; i < p.q_heads * D; i += kThreads)
+    if (span_of<C::keys>(p, s).steps == 0) {
+      for (int i = tid; i < p.q_heads * D; i += blockDim.x)
         store_row(p.a.out.ptr, p.a.type,
                   s * p.a.out.stride[0] + (i / D) * p.a.out.stride[1] + (i % D) * p.a.out.stride[2], 0.f);
       if (p.a.lse)
-        for (int i = tid; i < p.q_heads; i += kThreads) p.a.lse[s * p.q_heads + i] = -INFINITY;
+        for (int i = tid; i < p.q_heads; i += blockDim.x) p.a.lse[s * p.q_heads + i] = -INFINITY;
     }
-  if (begin >= end) return;
-
-  // the sequence that holds tile `begin`
+  const int64_t nominal0 = per * blockIdx.x, nominal1 = nominal0 + per;
+  if (nominal0 >= total) return;
+  if (nominal1 >= total && tid == 0) s_cut[1] = Cut{total, p.a.seqs, total, total, total};
   int64_t before = 0;
-  for (int64_t base = 0;; base += kThreads) {
+  for (int64_t base = 0; before <= nominal1 && base < p.a.seqs; base += blockDim.x) {
     const int64_t s = base + tid;
-    const int64_t n = s < p.a.seqs ? span_of<C::tile>(p, s).tiles * units : 0;
+    const int steps = s < p.a.seqs ? span_of<C::keys>(p, s).steps : 0;
+    const int64_t n = steps * units;
     int64_t sum = n;
     for (int d = 1; d < 32; d <<= 1) {
       const int64_t up = __shfl_up_sync(~0u, sum, d);
@@ -211,156 +364,146 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Params p) {
     }
     __syncthreads();
     if (lane == 31) s_scan[warp] = sum;
-    if (tid == 0) s_found[0] = -1;
     __syncthreads();
-    int64_t here = before;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) here += s_scan[w];
+    sum += before;
+    for (int w = 0; w < W; ++w) {
+      if (w < warp) sum += s_scan[w];
       before += s_scan[w];
     }
-    if (begin >= here + sum - n && begin < here + sum) {
-      s_found[0] = s;
-      s_found[1] = here + sum - n;
+    for (int k = 0; k < 2; ++k) {
+      const int64_t b = k ? nominal1 : nominal0, from = sum - n;
+      if (b >= from && b < sum) {
+        const int64_t x = from + (b - from) / steps * steps;
+        s_cut[k] = Cut{snapped(b, x, x + steps, near), s, from, x, x + steps};
+      }
     }
-    __syncthreads();
-    if (s_found[0] >= 0) break;
   }
-  int64_t seq = s_found[0], seq_begin = s_found[1];
-  Span sp = span_of<C::tile>(p, seq);
+  __syncthreads();
+  const int64_t begin = s_cut[0].at, end = s_cut[1].at;
+  if (begin >= end) return;
 
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (C::NST * C::stage) + lane * 16;
-  const uint32_t sq = (uint32_t)__cvta_generic_to_shared(smem) + C::ring;
+  // ---- this warp's share of it
+  const int64_t wb = begin + (end - begin) * warp / W, we = begin + (end - begin) * (warp + 1) / W;
+  int64_t seq = s_cut[0].seq, seq_begin = s_cut[0].seq_begin;
+  Span sp = span_of<C::keys>(p, seq);
+  if (lane < 2) s_seg[2 * warp + lane] = -1;
+
+  const int warp_bytes = C::kv + C::q_row * p.q_rows;
+  uint8_t *own = smem + warp * warp_bytes;
+  const uint32_t slots = (uint32_t)__cvta_generic_to_shared(own) + lane * 16;
+  // query row g in fragment order; lanes beyond the tile's rows repeat its last one, their results go nowhere
+  const uint32_t sq = (uint32_t)__cvta_generic_to_shared(own) + C::kv + min(g, p.q_rows - 1) * 64 + t * 16;
+  const int q_step = p.q_rows * 64;
   const bool paged16 = ps % 16 == 0;
   const uint8_t *kbase = static_cast<const uint8_t *>(p.pool.k), *vbase = static_cast<const uint8_t *>(p.pool.v);
   const int64_t kslot = p.pool.k_stride[2] * C::es, vslot = p.pool.v_stride[2] * C::es;
+  const int64_t kpage = p.pool.k_stride[0] * C::es, vpage = p.pool.v_stride[0] * C::es;
 
-  for (int64_t at = begin; at < end;) {
-    while (at >= seq_begin + sp.tiles * units) {  // next sequence with keys
-      seq_begin += sp.tiles * units;
-      sp = span_of<C::tile>(p, ++seq);
+  for (int64_t at = wb; at < we;) {
+    while (at >= seq_begin + sp.steps * units) {  // next sequence with keys
+      seq_begin += sp.steps * units;
+      sp = span_of<C::keys>(p, ++seq);
     }
-    const int64_t off = at - seq_begin, unit = off / sp.tiles;
-    const int tile0 = (int)(off - unit * sp.tiles);
+    const int64_t off = at - seq_begin, unit = off / sp.steps;
+    const int step0 = (int)(off - unit * sp.steps);
     const int h = (int)(unit / p.qtiles), qt = (int)(unit % p.qtiles);
-    const int64_t seg_begin = seq_begin + unit * sp.tiles, seg_end = seg_begin + sp.tiles;
-    const int n = (int)((seg_end < end ? seg_end : end) - at);
+    const int64_t seg_begin = seq_begin + unit * sp.steps, seg_end = seg_begin + sp.steps;
+    const int n = (int)((seg_end < we ? seg_end : we) - at);
     const int rows = min(kQT, p.group - qt * kQT), head0 = h * p.group + qt * kQT;
     const int32_t *table = p.a.page_table + seq * p.a.table_stride;
-    const int key0 = sp.start + tile0 * C::tile + warp * C::keys;
+    const int key0 = sp.start + step0 * C::keys;
+    const uint8_t *kh = kbase + h * p.pool.k_stride[1] * C::es, *vh = vbase + h * p.pool.v_stride[1] * C::es;
 
-    // ---- copies of one warp step: 16-byte pieces of K, then of V
-    uint64_t present = 0;  // 16 bits per ring stage: which of its keys there are
-    auto entry_of = [&](int key) -> int { return key < sp.len ? table[key / ps] : 0; };
-    int next_entry = paged16 ? entry_of(key0) : 0;
-    auto issue = [&](int i) {
-      const int key = key0 + i * C::tile;
-      const uint32_t st = ring + (i % C::NST) * C::stage;
-      uint32_t mask = 0;
-      if (i < n && key < sp.len) {
-        const int hi = min(sp.len - key, C::keys), lo = min(max(sp.first - key, 0), C::keys);
-        mask = ((1u << hi) - 1) & ~((1u << lo) - 1);
-        int64_t koff, voff;  // of key `key` (paged16), or of this lane's key
-        if (paged16) {
-          const int e = next_entry;
-          if (e < 0 || e >= p.pool.num_pages) {
-            if (lane == 0) serve::set_status(p.status, 8);
-            mask = 0;
-          }
-          const int64_t page = mask ? e : 0;
-          const int in = key % ps;
-          koff = (page * p.pool.k_stride[0] + h * p.pool.k_stride[1]) * C::es + in * kslot;
-          voff = (page * p.pool.v_stride[0] + h * p.pool.v_stride[1]) * C::es + in * vslot;
-          next_entry = entry_of(key + C::tile);
-        } else {
-          int e = 0;
-          const int mykey = key + (lane % C::keys);
-          const bool want = mask >> (lane % C::keys) & 1;
-          if (want) e = table[mykey / ps];
-          const bool ok = want && e >= 0 && e < p.pool.num_pages;
-          if (want && !ok) serve::set_status(p.status, 8);
-          mask = __ballot_sync(~0u, ok) & ((1u << C::keys) - 1);
-          const int64_t page = ok ? e : 0;
-          const int in = ok ? mykey % ps : 0;
-          koff = (page * p.pool.k_stride[0] + h * p.pool.k_stride[1]) * C::es + in * kslot;
-          voff = (page * p.pool.v_stride[0] + h * p.pool.v_stride[1]) * C::es + in * vslot;
-        }
-        if (mask) {
+    // ---- places of a step's keys: a page entry per 16 keys, or one per key
+    constexpr int NS = C::keys / C::sub;
+    int entry[NS];  // paged16: of each 16 keys; else entry[0], of key lane % keys
+    auto look_up = [&](int key) {
+      if (paged16) {
 #pragma unroll
-          for (int nt = 0; nt < C::NT; ++nt) {
-            const int k = nt * 8 + g;
-            const uint8_t *src = kbase + (paged16 ? koff + k * kslot : __shfl_sync(~0u, koff, k));
-            const bool ok = mask >> k & 1;
-#pragma unroll
-            for (int j = 0; j < C::KJ; ++j) {
-              const int piece = t + 4 * j;
-              const bool in = ok && piece * C::epc < D;
-              copy16(st + (nt * C::KJ + j) * 512, in ? src + piece * 16 : kbase, in);
-            }
-          }
-#pragma unroll
-          for (int kk = 0; kk < 2 * C::NT; ++kk) {
-            const int k = (kk / 2) * 8 + 2 * t + kk % 2;
-            const uint8_t *src = vbase + (paged16 ? voff + k * vslot : __shfl_sync(~0u, voff, k));
-            const bool ok = mask >> k & 1;
-#pragma unroll
-            for (int j = 0; j < C::VJ; ++j) {
-              const int piece = g + 8 * j;
-              const bool in = ok && piece * C::epc < D;
-              copy16(st + (C::NT * C::KJ + kk * C::VJ + j) * 512, in ? src + piece * 16 : vbase, in);
-            }
-          }
-        }
+        for (int i = 0; i < NS; ++i)
+          entry[i] = key + i * 16 < sp.len ? table[page_of(p, key + i * 16)] : 0;
+      } else {
+        const int k = key + lane % C::keys;
+        entry[0] = k >= sp.first && k < sp.len ? table[page_of(p, k)] : 0;
       }
-      const int sh = (i % C::NST) * 16;
-      present = (present & ~(0xffffull << sh)) | ((uint64_t)mask << sh);
-      asm volatile("cp.async.commit_group;");
     };
-    for (int i = 0; i < C::NST - 1; ++i) issue(i);
+    // present keys of the step at `key`, by entries as looked up
+    auto present_of = [&](int key) -> uint32_t {
+      const int hi = min(sp.len - key, C::keys), lo = min(max(sp.first - key, 0), C::keys);
+      uint32_t mask = (uint32_t)((1ull << hi) - 1) & ~(uint32_t)((1ull << lo) - 1);
+      bool bad = false;
+      if (paged16) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+          if (key + i * 16 < sp.len && (uint32_t)entry[i] >= (uint32_t)p.pool.num_pages) {
+            bad = true;
+            mask &= ~(0xffffu << (16 * i));
+            entry[i] = 0;
+          }
+      } else {
+        const bool ok = (uint32_t)entry[0] < (uint32_t)p.pool.num_pages;
+        const uint32_t good = __ballot_sync(~0u, ok);
+        bad = !ok;
+        mask &= good;
+        if (!ok) entry[0] = 0;
+      }
+      if (bad) serve::set_status(p.status, 8);
+      return mask;
+    };
+    // the row of key k8 + k of a step; k8 a constant multiple of 8, k below 8
+    auto row_of = [&](const uint8_t *base, int64_t page, int64_t slot, int key, int k8, int k) -> const uint8_t * {
+      if (paged16) {
+        const int first = key + k8 / 16 * 16;
+        return base + entry[k8 / 16] * page + (first - page_of(p, first) * ps + k8 % 16 + k) * slot;
+      }
+      const int e = __shfl_sync(~0u, entry[0], k8 + k), kk = key + k8 + k;
+      return base + e * page + (kk - page_of(p, kk) * ps) * slot;
+    };
+    auto copy_k = [&](int key, uint32_t mask) {
+#pragma unroll
+      for (int nt = 0; nt < C::NT; ++nt) {
+        const int k = nt * 8 + g;
+        const uint8_t *src = row_of(kh, kpage, kslot, key, nt * 8, g) + t * 16;
+        const bool ok = mask >> k & 1;
+        if (!ok) src = kbase;
+#pragma unroll
+        for (int j = 0; j < C::KJ; ++j)
+          copy16(slots + (nt * C::KJ + j) * 512, src + j * 64, ok && (t + 4 * j) * C::epc < D);
+      }
+    };
+    auto copy_v = [&](int key, uint32_t mask) {
+#pragma unroll
+      for (int kk = 0; kk < 2 * C::NT; ++kk) {
+        const int k = (kk / 2) * 8 + 2 * t + kk % 2;
+        const uint8_t *src = row_of(vh, vpage, vslot, key, kk / 2 * 8, 2 * t + kk % 2) + g * 16;
+        const bool ok = mask >> k & 1;
+        if (!ok) src = vbase;
+#pragma unroll
+        for (int j = 0; j < C::VJ; ++j)
+          copy16(slots + (C::k_slots + kk * C::VJ + j) * 512, src + j * 128, ok && (g + 8 * j) * C::epc < D);
+      }
+    };
+    look_up(key0);
+    uint32_t mask = present_of(key0);
+    copy_k(key0, mask);
+    asm volatile("cp.async.commit_group;");
+    copy_v(key0, mask);
+    asm volatile("cp.async.commit_group;");
 
     // ---- the query tile, split into parts, in fragment order
-    auto q_at = [&](int r, int d) {
-      return r < rows && d < D ? load_row(p.a.q.ptr, p.a.type,
-                                          seq * p.a.q.stride[0] + (head0 + r) * p.a.q.stride[1] + d * p.a.q.stride[2])
-                               : 0.f;
-    };
-    for (int r = warp; r < kQT; r += kWarps) {
-      // fp16 parts: rows are scaled by a power of two to below 2, so that no
-      // part overflows and the tails stay above fp16's smallest values
-      float up = 1.f;
-      if (MODE == kF16Wide) {
-        float top = 0.f;
-        for (int d = lane; d < D; d += 32) top = fmaxf(top, fabsf(q_at(r, d)));
-        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-        const int e = (int)(__float_as_uint(top) >> 23) - 127;  // floor(log2(top)) of a normal number
-        if (e > -120 && e < 127) up = __uint_as_float((uint32_t)(e + 127) << 23);
-      }
-      if (lane == 0) s_scale[r] = up;
+    const int64_t q0 = seq * p.a.q.stride[0] + (head0 + min(g, rows - 1)) * p.a.q.stride[1];
+    float up = 1.f;
+    if (g < p.q_rows) {
+      const uint32_t group = p.q_rows == kQT ? ~0u : (1u << (4 * p.q_rows)) - 1;
+      if (p.a.type == SC_TYPE_F32)
+        up = fill_q<MODE, DP>(static_cast<const float *>(p.a.q.ptr) + q0, p, t, sq, q_step, group);
+      else if (p.a.type == SC_TYPE_F16)
+        up = fill_q<MODE, DP>(static_cast<const __half *>(p.a.q.ptr) + q0, p, t, sq, q_step, group);
+      else
+        up = fill_q<MODE, DP>(static_cast<const __nv_bfloat16 *>(p.a.q.ptr) + q0, p, t, sq, q_step, group);
     }
-    if (MODE == kF16Wide) __syncthreads();
-    for (int i = tid; i < C::KJ * 32; i += kThreads) {
-      const int l = i % 32, r = l / 4, d0 = (l % 4 + 4 * (i / 32)) * C::epc;
-      float x[C::epc];
-#pragma unroll
-      for (int e = 0; e < C::epc; ++e) {
-        x[e] = q_at(r, d0 + e);
-        if (MODE == kF16Wide) x[e] *= 1.f / s_scale[r];
-      }
-#pragma unroll
-      for (int part = 0; part < C::parts; ++part) {
-        uint32_t w[4];
-        for (int e = 0; e < 4; ++e) {
-          if (C::f32)
-            w[e] = part ? tf32_tail(x[e]) : tf32_head(x[e]);
-          else
-            w[e] = pack2<MODE>(x[(2 * e) % C::epc], x[(2 * e + 1) % C::epc]);
-        }
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(sq + ((i / 32) * C::parts + part) * 512 + l * 16),
-                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                     : "memory");
-      }
-    }
-    __syncthreads();
-    const float c = p.scale_log2 * s_scale[g];
+    __syncwarp();
+    const float c = p.scale_log2 * __shfl_sync(~0u, up, 4 * min(g, p.q_rows - 1));
 
     // ---- one pass over the keys
     float m = -INFINITY, l = 0.f;
@@ -368,21 +511,19 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Params p) {
     float o[ON][2];
 #pragma unroll
     for (int i = 0; i < ON; ++i) o[i][0] = o[i][1] = 0.f;
+    if (n > 1) look_up(key0 + C::keys);
     for (int i = 0; i < n; ++i) {
-      issue(i + C::NST - 1);
-      asm volatile("cp.async.wait_group %0;" ::"n"(C::NST - 1) : "memory");
-      const uint32_t mask = (uint32_t)(present >> ((i % C::NST) * 16)) & 0xffffu;
-      if (!mask) continue;
-      const uint32_t st = ring + (i % C::NST) * C::stage;
+      const int next = key0 + (i + 1) * C::keys;
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
       float s[C::NT][2][4] = {};
 #pragma unroll
       for (int j = 0; j < C::KJ; ++j) {
         uint4 q[C::parts];
 #pragma unroll
-        for (int part = 0; part < C::parts; ++part) q[part] = lds(sq + (j * C::parts + part) * 512 + lane * 16);
+        for (int part = 0; part < C::parts; ++part) q[part] = lds(sq + (j * C::parts + part) * q_step);
 #pragma unroll
         for (int nt = 0; nt < C::NT; ++nt) {
-          const uint4 k = lds(st + (nt * C::KJ + j) * 512);
+          const uint4 k = lds(slots + (nt * C::KJ + j) * 512);
           if (C::f32) {
             const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
             const uint32_t qh[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
@@ -405,7 +546,13 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Params p) {
           }
         }
       }
-      // running maximum and sum; a lane has query g and keys 2t, 2t+1 (+8)
+      const uint32_t now = mask;
+      if (i + 1 < n) {
+        mask = present_of(next);
+        copy_k(next, mask);
+      }
+      asm volatile("cp.async.commit_group;");
+      // running maximum and sum; a lane has query g and keys 2t, 2t+1 of every 8
       float x[C::NT][2], top = -INFINITY;
 #pragma unroll
       for (int nt = 0; nt < C::NT; ++nt)
@@ -413,7 +560,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Params p) {
         for (int e = 0; e < 2; ++e) {
           x[nt][e] = s[nt][0][e] + s[nt][1][e];
           if (C::parts > 1) x[nt][e] += s[nt][0][2 + e] + s[nt][1][2 + e];
-          if (!(mask >> (nt * 8 + 2 * t + e) & 1)) x[nt][e] = -INFINITY;
+          if (!(now >> (nt * 8 + 2 * t + e) & 1)) x[nt][e] = -INFINITY;
           top = fmaxf(top, x[nt][e]);
         }
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
@@ -423,160 +570,202 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Params p) {
       const float shrink = ex2(m - ref);
       m = top;
       l *= shrink;
-      uint32_t pa[C::NT][4];  // P as A fragments: one per 8 keys (f32) or pa[0]
 #pragma unroll
-      for (int nt = 0; nt < C::NT; ++nt) {
+      for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           x[nt][e] = ex2(fmaf(x[nt][e], c, -ref));
           l += x[nt][e];
         }
-      }
-      if (C::f32) {
+      constexpr int PN = C::f32 ? C::NT : C::NT / 2;  // A fragments of P: of 8 keys (f32) or 16
+      uint32_t pa[PN][4], p3[PN][2];
 #pragma unroll
-        for (int nt = 0; nt < C::NT; ++nt) {
-          pa[nt][0] = tf32_head(x[nt][0]);
-          pa[nt][1] = tf32_tail(x[nt][0]);
-          pa[nt][2] = tf32_head(x[nt][1]);
-          pa[nt][3] = tf32_tail(x[nt][1]);
+      for (int k = 0; k < PN; ++k) {
+        if (C::f32) {
+          pa[k][0] = tf32_head(x[k][0]);
+          pa[k][1] = tf32_tail(x[k][0]);
+          pa[k][2] = tf32_head(x[k][1]);
+          pa[k][3] = tf32_tail(x[k][1]);
+        } else {
+          constexpr int two = C::f32 ? 0 : 1;
+          float(&xa)[2] = x[two * 2 * k], (&xb)[2] = x[two * (2 * k + 1)];
+          pa[k][0] = pack2<MODE>(xa[0], xa[1]);
+          pa[k][2] = pack2<MODE>(xb[0], xb[1]);
+          pa[k][1] = pack2<MODE>(xa[0], xa[1]);
+          pa[k][3] = pack2<MODE>(xb[0], xb[1]);
+          if (MODE == kBF16Wide) {
+            p3[k][0] = pack2<MODE>(xa[0], xa[1]);
+            p3[k][1] = pack2<MODE>(xb[0], xb[1]);
+          }
         }
-      } else {
-        pa[0][0] = pack2<MODE>(x[0][0], x[0][1]);
-        pa[0][2] = pack2<MODE>(x[C::NT - 1][0], x[C::NT - 1][1]);
-        pa[0][1] = pack2<MODE>(x[0][0], x[0][1]);
-        pa[0][3] = pack2<MODE>(x[C::NT - 1][0], x[C::NT - 1][1]);
       }
-      uint32_t p3a = 0, p3b = 0;
-      if (MODE == kBF16Wide) {
-        p3a = pack2<MODE>(x[0][0], x[0][1]);
-        p3b = pack2<MODE>(x[C::NT - 1][0], x[C::NT - 1][1]);
-      }
-      const uint32_t sv = st + C::NT * C::KJ * 512;
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
 #pragma unroll
       for (int j = 0; j < C::VJ; ++j) {
         uint32_t v[2 * C::NT][4];
 #pragma unroll
         for (int kk = 0; kk < 2 * C::NT; ++kk) {
-          const uint4 w = lds(sv + (kk * C::VJ + j) * 512);
+          const uint4 w = lds(slots + (C::k_slots + kk * C::VJ + j) * 512);
           v[kk][0] = w.x, v[kk][1] = w.y, v[kk][2] = w.z, v[kk][3] = w.w;
         }
 #pragma unroll
         for (int e = 0; e < C::epc; ++e) {
           float acc[4] = {};
-          if (C::f32) {
 #pragma unroll
-            for (int nt = 0; nt < C::NT; ++nt) {
-              const float v0 = __uint_as_float(v[2 * nt][e % 4]), v1 = __uint_as_float(v[2 * nt + 1][e % 4]);
-              mma<MODE>(acc, pa[nt][0], pa[nt][1], pa[nt][2], pa[nt][3], tf32_head(v0), tf32_head(v1));
-              mma<MODE>(acc, pa[nt][0], pa[nt][1], pa[nt][2], pa[nt][3], tf32_tail(v0), tf32_tail(v1));
+          for (int k = 0; k < PN; ++k) {
+            if (C::f32) {
+              const float v0 = __uint_as_float(v[2 * k][e % 4]), v1 = __uint_as_float(v[2 * k + 1][e % 4]);
+              mma<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], tf32_head(v0), tf32_head(v1));
+              mma<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], tf32_tail(v0), tf32_tail(v1));
+            } else {
+              const uint32_t sel = e % 2 ? 0x7632 : 0x5410;
+              constexpr int two = C::f32 ? 0 : 4;
+              const uint32_t b0 = __byte_perm(v[two * k][e / 2], v[two * k + 1][e / 2], sel);
+              const uint32_t b1 = __byte_perm(v[two * k + two / 2][e / 2], v[two * k + two / 2 + 1][e / 2], sel);
+              mma<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], b0, b1);
+              if (MODE == kBF16Wide) mma<MODE>(acc, p3[k][0], 0, p3[k][1], 0, b0, b1);
             }
-          } else {
-            const uint32_t sel = e % 2 ? 0x7632 : 0x5410;
-            const uint32_t b0 = __byte_perm(v[0][e / 2], v[1][e / 2], sel);
-            const uint32_t b1 = __byte_perm(v[2 * C::NT - 2][e / 2], v[2 * C::NT - 1][e / 2], sel);
-            mma<MODE>(acc, pa[0][0], pa[0][1], pa[0][2], pa[0][3], b0, b1);
-            if (MODE == kBF16Wide) mma<MODE>(acc, p3a, 0, p3b, 0, b0, b1);
           }
           float *oo = o[j * C::epc + e];
           oo[0] = fmaf(oo[0], shrink, acc[0] + acc[2]);
           oo[1] = fmaf(oo[1], shrink, acc[1] + acc[3]);
         }
       }
+      if (i + 1 < n) {
+        copy_v(next, mask);
+        if (i + 2 < n) look_up(next + C::keys);
+      }
+      asm volatile("cp.async.commit_group;");
     }
-
-    // ---- join the warps
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     l += __shfl_xor_sync(~0u, l, 1);
     l += __shfl_xor_sync(~0u, l, 2);
-    if (t == 0) s_m[warp][g] = m, s_l[warp][g] = l;
-    __syncwarp();  // every lane has read its last stage before O goes into the warp's ring
-    float *so = reinterpret_cast<float *>(smem) + warp * (C::NST * C::stage / 4);
+    __syncwarp();  // every lane has read its last slots
+    if (at == seg_begin && at + n == seg_end) {
+      if (g < rows) {
+        const float scale = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int j = 0; j < C::VJ; ++j)
+        for (int j = 0; j < C::VJ; ++j)
 #pragma unroll
-      for (int e = 0; e < C::epc; ++e)
+          for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int d = (8 * j + 2 * t + k) * C::epc + e;
-          if (d < DP) so[g * C::o_row + d] = o[j * C::epc + e][k];
-        }
-    __syncthreads();
-    const float *all = reinterpret_cast<const float *>(smem);
-    const bool whole = at == seg_begin && at + n == seg_end;
-    float *record = p.partials + ((int64_t)blockIdx.x * 2 + (at == seg_begin)) * C::record;
-    if (tid < rows) {
-      float top = -INFINITY, sum = 0.f;
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][tid]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      for (int w = 0; w < kWarps; ++w) sum += s_l[w][tid] * ex2(s_m[w][tid] - ref);
-      s_top[tid] = ref;
-      s_sum[tid] = sum;
-      if (whole) {
-        if (p.a.lse) p.a.lse[seq * p.q_heads + head0 + tid] = (ref + log2f(sum)) * 0.69314718055994531f;
-      } else {
-        record[kQT * DP + tid] = top;
-        record[kQT * DP + kQT + tid] = sum;
+            for (int e = 0; e < C::epc; e += 4) {
+              const int d = (8 * j + 2 * t + k) * C::epc + e;
+              const int b = j * C::epc + e;
+              if (d < D)
+                store4(p, seq, head0 + g, d,
+                       make_float4(o[b][k] * scale, o[b + 1][k] * scale, o[b + 2][k] * scale, o[b + 3][k] * scale));
+            }
+        if (p.a.lse && t == 0) p.a.lse[seq * p.q_heads + head0 + g] = lse_of(m == -INFINITY ? 0.f : m, l);
       }
-    }
-    __syncthreads();
-    for (int i = tid; i < rows * D; i += kThreads) {
-      const int r = i / D, d = i - r * D;
-      float y = 0.f;
+    } else {
+      // the last piece of a run stays in the warp's slots, an earlier one goes to the workspace
+      const int tail = at + n == we;
+      float *to = tail ? reinterpret_cast<float *>(own) : p.heads + ((int64_t)blockIdx.x * W + warp) * C::piece;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-        y += all[w * (C::NST * C::stage / 4) + r * C::o_row + d] * ex2(s_m[w][r] - s_top[r]);
-      if (whole)
-        store_row(p.a.out.ptr, p.a.type,
-                  seq * p.a.out.stride[0] + (head0 + r) * p.a.out.stride[1] + d * p.a.out.stride[2],
-                  s_sum[r] == 0.f ? 0.f : y / s_sum[r]);
-      else
-        record[r * DP + d] = y;
-    }
-    if (!whole) {
-      // the last of the segment's blocks adds their records up in block order
-      const int first = (int)(seg_begin / per), last = (int)((seg_end - 1) / per);
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        int *word = p.arrivals + seq * units + unit;
-        s_last = atomicAdd(word, 1) == last - first;
-        if (s_last) *word = 0;
-      }
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        auto rec = [&](int b) { return p.partials + ((int64_t)b * 2 + (b == first)) * C::record; };
-        float *w = reinterpret_cast<float *>(smem);  // [blocks of the segment][kQT] weights
-        const int parts = last - first + 1;
-        for (int i = tid; i < parts * rows; i += kThreads)
-          w[(i / rows) * kQT + i % rows] = __ldcg(rec(first + i / rows) + kQT * DP + i % rows);
-        __syncthreads();
-        if (tid < rows) {
-          float top = -INFINITY, sum = 0.f;
-          for (int b = 0; b < parts; ++b) top = fmaxf(top, w[b * kQT + tid]);
-          const float ref = top == -INFINITY ? 0.f : top;
-          for (int b = 0; b < parts; ++b) {
-            const float f = ex2(w[b * kQT + tid] - ref);
-            w[b * kQT + tid] = f;
-            sum += f * __ldcg(rec(first + b) + kQT * DP + kQT + tid);
+      for (int j = 0; j < C::VJ; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < C::epc; e += 4) {
+            const int d = (8 * j + 2 * t + k) * C::epc + e, b = j * C::epc + e;
+            if (d < DP && g < rows)
+              *reinterpret_cast<float4 *>(to + g * C::o_row + d) =
+                  make_float4(o[b][k], o[b + 1][k], o[b + 2][k], o[b + 3][k]);
           }
-          s_sum[tid] = sum;
-          if (p.a.lse) p.a.lse[seq * p.q_heads + head0 + tid] = (ref + log2f(sum)) * 0.69314718055994531f;
-        }
-        __syncthreads();
-        for (int i = tid; i < rows * D; i += kThreads) {
-          const int r = i / D, d = i - r * D;
-          float y = 0.f;
-#pragma unroll 8
-          for (int b = 0; b < parts; ++b) y += w[b * kQT + r] * __ldcg(rec(first + b) + r * DP + d);
-          store_row(p.a.out.ptr, p.a.type,
-                    seq * p.a.out.stride[0] + (head0 + r) * p.a.out.stride[1] + d * p.a.out.stride[2],
-                    s_sum[r] == 0.f ? 0.f : y / s_sum[r]);
-        }
+      if (t == 0) {
+        to[kQT * C::o_row + g] = m;
+        to[kQT * C::o_row + kQT + g] = l;
+      }
+      if (lane == 0) {
+        const int i = 2 * warp + tail;
+        s_seg[i] = seg_begin, s_end[i] = seg_end, s_seq[i] = seq, s_unit[i] = unit;
+      }
+    }
+    at += n;
+  }
+
+  // ---- the block's pieces, one warp per segment and row
+  __syncthreads();
+  if (warp == 0) {
+    const bool has = lane < 2 * W && s_seg[lane] >= 0;
+    const uint32_t valid = __ballot_sync(~0u, has), earlier = valid & ((1u << lane) - 1);
+    const bool leads = has && (!earlier || s_seg[31 - __clz(earlier)] != s_seg[lane]);
+    const uint32_t leaders = __ballot_sync(~0u, leads);
+    if (lane == 0) s_masks[0] = valid, s_masks[1] = leaders;
+  }
+  __syncthreads();
+  const uint32_t valid = s_masks[0];
+  constexpr int ND = (DP + 127) / 128;
+  auto write_row = [&](int64_t seq, int head, const float4 (&y)[ND], float ref, float sum) {
+    const float scale = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < ND; ++k) {
+      const int d = 4 * lane + 128 * k;
+      if (d < D)
+        store4(p, seq, head, d, make_float4(y[k].x * scale, y[k].y * scale, y[k].z * scale, y[k].w * scale));
+    }
+    if (p.a.lse && lane == 0) p.a.lse[seq * p.q_heads + head] = lse_of(ref, sum);
+  };
+  const int groups = __popc(s_masks[1]);
+  for (int task = warp; task < groups * p.q_rows; task += W) {
+    const int r = task % p.q_rows;
+    uint32_t leaders = s_masks[1];
+    for (int k = task / p.q_rows; k; --k) leaders &= leaders - 1;
+    const int lead = __ffs(leaders) - 1;
+    leaders &= leaders - 1;
+    const uint32_t members = valid & ~((1u << lead) - 1) & (leaders ? (1u << (__ffs(leaders) - 1)) - 1 : ~0u);
+    const int64_t unit = s_unit[lead];
+    const int qt = (int)(unit % p.qtiles), head = (int)(unit / p.qtiles) * p.group + qt * kQT + r;
+    if (qt * kQT + r >= p.group) continue;
+    float4 y[ND];
+    float ref, sum;
+    add_up<DP>(PieceList{members, p.heads + (int64_t)blockIdx.x * W * C::piece, smem, C::piece, warp_bytes}, r, y, ref,
+               sum);
+    if (s_seg[lead] >= begin && s_end[lead] <= end) {
+      write_row(s_seq[lead], head, y, ref, sum);
+    } else {
+      float *rec = p.records + ((int64_t)blockIdx.x * 2 + (s_seg[lead] >= begin)) * C::piece;
+#pragma unroll
+      for (int k = 0; k < ND; ++k)
+        if (4 * lane + 128 * k < DP) *reinterpret_cast<float4 *>(rec + r * C::o_row + 4 * lane + 128 * k) = y[k];
+      if (lane == 0) {
+        rec[kQT * C::o_row + r] = sum == 0.f ? -INFINITY : ref;
+        rec[kQT * C::o_row + kQT + r] = sum;
+      }
+    }
+  }
+
+  // ---- segments that pass this run's ends: the last block to arrive adds the records up
+  for (int k = 0; k < 2; ++k) {
+    const Cut cut = s_cut[k];
+    const int64_t x = cut.seg_begin, y_end = cut.seg_end;
+    if (cut.at <= x || cut.at >= y_end || (k && x < begin)) continue;
+    // the blocks of the segment: cuts inside it, by the same rule as above
+    int64_t lo = x / per + 1, hi = (y_end + per - 1) / per - 1;
+    while (snapped(lo * per, x, y_end, near) == x) ++lo;
+    while (snapped(hi * per, x, y_end, near) == y_end) --hi;
+    const int first = (int)lo - 1, last = (int)hi;
+    const int64_t unit = (x - cut.seq_begin) / (y_end - x);
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      int *word = p.arrivals + cut.seq * units + unit;
+      s_last = atomicAdd(word, 1) == last - first;
+      if (s_last) *word = 0;
+    }
+    __syncthreads();
+    if (s_last) {
+      __threadfence();
+      const int qt = (int)(unit % p.qtiles), rows = min(kQT, p.group - qt * kQT);
+      for (int r = warp; r < rows; r += W) {
+        float4 y[ND];
+        float ref, sum;
+        add_up<DP>(RecordList{p.records, C::piece, first, last}, r, y, ref, sum);
+        write_row(cut.seq, (int)(unit / p.qtiles) * p.group + qt * kQT + r, y, ref, sum);
       }
     }
     __syncthreads();
-    at += n;
   }
 }
 

@@ -101,10 +101,14 @@ class _Handle:
         if v:
             raise ScError(SC_ERR_DEVICE, f"a kernel skipped entries that were out of range (status {v})")
 
+    def _own(self, h: ctypes.c_void_p) -> None:
+        self._h = h
+        self._release = getattr(lib(), self._free)  # module globals may be gone when the interpreter ends
+
     def __del__(self):
-        if self._h and self._h.value:
-            getattr(lib(), self._free)(self._h)
-            self._h = ctypes.c_void_p()
+        if self._h is not None:
+            self._release(self._h)
+            self._h = None
 
 
 class RotaryTable:
@@ -148,7 +152,7 @@ class PagedKVCache(_Handle):
                           *k.stride()[:3], *v.stride()[:3], _TYPES[k.dtype])
         h = ctypes.c_void_p()
         _check(lib().sc_kv_cache_create(pool, self.device, ctypes.byref(h)))
-        self._h = h
+        self._own(h)
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.float32,
@@ -227,7 +231,7 @@ class DecodeAttention(_Handle):
         self.device = cache.device
         h = ctypes.c_void_p()
         _check(lib().sc_attn_create(cache._h, q_heads, max_seqs, scale or 0.0, window, ctypes.byref(h)))
-        self._h = h
+        self._own(h)
 
     def attend(self, q, page_table, seq_lens, out=None, return_lse: bool = False, stream=None):
         """out[s] = softmax(scale q[s] k^T) v over the ``seq_lens[s]`` first
@@ -296,7 +300,7 @@ class LowRankAdapters(_Handle):
             self.device, self.in_features, self.out_features, n, i64(*ranks), _TYPES[dtype],
             vp(*[a.data_ptr() for a in down]), i64(*dl), vp(*[b.data_ptr() for b in up]), i64(*ul),
             (ctypes.c_float * n)(*[float(x) for x in scales]), stream, ctypes.byref(h)))
-        self._h = h
+        self._own(h)
         self.ranks = ranks
         self._scratch = (-1, 0)
 
