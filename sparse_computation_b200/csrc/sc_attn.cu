@@ -16,12 +16,12 @@ struct Variant {
   int warps, smem, keys, piece;
 };
 
-// As many warps as registers (16, or 8 from head_dim 129 on) and shared
-// memory allow: each has its K and V slots and its query tile.
+// As many warps as registers (Cfg::max_warps) and shared memory (a query tile
+// or a piece each) allow.
 template <int MODE, int DP>
 Variant variant(int q_rows, int smem_limit) {
   using C = Cfg<MODE, DP>;
-  const int per_warp = C::kv + C::q_row * q_rows;
+  const int per_warp = C::warp_bytes(q_rows);
   Variant v{attend_kernel<MODE, DP>, 0, 0, C::keys, C::piece};
   cudaFuncAttributes attr;
   cuda_check(cudaFuncGetAttributes(&attr, v.kernel), "kernel attributes");
@@ -78,6 +78,7 @@ int sc_attn_create(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, 
   p->scale = (float)(scale > 0 ? scale : 1.0 / std::sqrt((double)pool.head_dim));
   p->qtiles = (int)((q_heads / pool.kv_heads + kQT - 1) / kQT);
   const int64_t segments = max_seqs * pool.kv_heads * p->qtiles;
+  // a run of one block is counted in 32 bits
   require(segments < INT32_MAX, SC_ERR_UNSUPPORTED, "max_seqs times heads reaches 2^31");
   p->q_rows = (int)std::min<int64_t>(q_heads / pool.kv_heads, kQT);
   // key / page_size for keys below 2^31: multiply by 2^(31 + bits) / page_size, rounded up
@@ -131,18 +132,21 @@ int sc_attn_decode(sc_attn *p, const sc_attn_args *a, void *stream) {
   require(a->q.ptr && a->out.ptr && a->page_table && a->seq_lens, SC_ERR_ARG,
           "null q, out, page table or lengths");
   require(a->table_cols >= 0 && a->table_stride >= 0, SC_ERR_ARG, "bad page table sizes");
-  const int64_t e = type_bytes(a->type);
+  const int64_t e = type_bytes(a->type), ce = type_bytes(p->pool.type);
   const int q_vec = a->q.stride[2] == 1 && a->q.stride[1] * e % 16 == 0 && a->q.stride[0] * e % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(a->q.ptr) % 16 == 0 && p->pool.head_dim % 8 == 0;
   const Variant &v = a->type == p->pool.type ? p->same : p->other;
   Params k{*a, p->pool, (int)p->q_heads, (int)(p->q_heads / p->pool.kv_heads), p->qtiles, p->q_rows, v.warps,
-           p->page_mul, p->page_shift, q_vec, (float)(p->scale * 1.4426950408889634), p->window, p->status, p->arrivals,
+           p->page_mul, p->page_shift, q_vec, p->pool.k_stride[0] * ce, p->pool.k_stride[1] * ce, p->pool.k_stride[2] * ce,
+           p->pool.v_stride[0] * ce, p->pool.v_stride[1] * ce, p->pool.v_stride[2] * ce,
+           (float)(p->scale * 1.4426950408889634), p->window, p->status, p->arrivals,
            p->heads, p->records};
   // the most steps that these lengths can have; the true number is known on the device only
   int64_t keys = std::min<int64_t>(a->table_cols, INT32_MAX / p->pool.page_size) * p->pool.page_size;
   if (p->window) keys = std::min(keys, p->window + 15);
   const int64_t steps = std::max<int64_t>(1, (keys + v.keys - 1) / v.keys) * a->seqs * p->pool.kv_heads * p->qtiles;
   const int64_t blocks = std::min<int64_t>((steps + v.warps - 1) / v.warps, p->sms);
+  require(steps / blocks < INT32_MAX / 2, SC_ERR_UNSUPPORTED, "the table names more keys than one call can take");
   DeviceGuard dg(p->device);
   v.kernel<<<(unsigned)blocks, v.warps * 32, v.smem, static_cast<cudaStream_t>(stream)>>>(k);
   cuda_check(cudaGetLastError(), "launch decode attention");

@@ -17,12 +17,13 @@
 // run in any order and the columns of O may be any permutation, so each lane
 // takes whole 16-byte pieces: of K, piece t + 4j of key g (g = lane / 4,
 // t = lane % 4) is a B fragment of 2 k-steps; of V, piece g + 8j of keys
-// 2t, 2t+1 (+8) holds one column of O per element.  A lane therefore only
-// ever reads back what it copied itself: its cp.async slots in shared memory
-// need no barrier, only its own wait_group.  Each warp has one slot for K and
-// one for V; the next K is asked for as soon as the scores are done, the next
-// V after the product with P.  With 16 warps a SM and 8 KB a warp step that
-// keeps 64-128 KB in flight, more than latency times bandwidth asks for.
+// 2t, 2t+1 (+8) holds one column of O per element.  K and V go from global
+// memory straight into the registers that feed the matrix instructions: the
+// next K is asked for as soon as the scores are done, the next V after the
+// product with P.  At 8 KB a warp step and 12 or 16 warps a SM that is
+// 64-128 KB in flight, more than latency times bandwidth asks for.  (The same
+// through cp.async and shared memory was bound by the extra 16 shared loads a
+// step: 147 us against TODO at 131071 keys, 8 kv heads of 128, bf16.)
 //
 // Work.  All (sequence, kv head, query tile) segments are cut into steps of
 // kKeys keys and laid end to end.  Every block takes one equal, contiguous
@@ -43,7 +44,7 @@ namespace attn {
 
 using serve::to_f32;
 
-constexpr int kQT = 8, kMaxWarps = 16;
+constexpr int kQT = 8, kMaxWarps = 12;
 
 enum Mode { kTF32, kBF16, kBF16Wide, kF16, kF16Wide };
 
@@ -54,6 +55,7 @@ struct Params {
   int min_run;                         // fewest steps of a block
   uint32_t page_mul, page_shift;       // key / page_size = umulhi(key, mul) >> shift (mul 0: page_size 1)
   int q_vec;                           // query rows are contiguous and 16-byte aligned
+  int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;  // strides in bytes
   float scale_log2;                    // scale * log2(e)
   int64_t window;
   int *status;
@@ -69,15 +71,16 @@ struct Cfg {
   // 8-key columns of S per step: 8 KB of K and V (16 KB from head_dim 129 on)
   static constexpr int NT = f32 ? (DP > 64 ? 1 : 2) : (DP > 64 ? 2 : 4);
   static constexpr int KJ = DP / (4 * epc), VJ = (DP + 8 * epc - 1) / (8 * epc);
-  static constexpr int k_slots = NT * KJ, v_slots = 2 * NT * VJ, kv = (k_slots + v_slots) * 512;
   static constexpr int parts = MODE == kBF16Wide ? 3 : MODE == kBF16 || MODE == kF16 ? 1 : 2;  // of Q
   static constexpr int keys = NT * 8;
   static constexpr int sub = keys < 16 ? keys : 16;  // keys that lie in one page when page_size is a multiple of 16
   static constexpr int q_row = KJ * parts * 64;      // bytes of one query row in fragment order
-  static constexpr int max_warps = DP > 128 ? 8 : kMaxWarps;
+  static constexpr int max_warps = DP > 128 ? 8 : 12;  // by the registers of a step
+  static constexpr bool ahead = DP <= 128;  // registers suffice to load a step ahead
   static constexpr int o_row = DP + 4;               // floats; the pad spreads rows over the banks
   static constexpr int piece = kQT * o_row + 2 * kQT;  // O | m | l
-  static_assert(kv >= piece * 4, "a warp's slots hold its last piece");
+  // shared memory of a warp: its query tile, later its last piece
+  __host__ __device__ static constexpr int warp_bytes(int q_rows) { return (q_row * q_rows > piece * 4 ? q_row * q_rows : piece * 4); }
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -86,8 +89,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool ok) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0));
+// 16 bytes that are read once: past L1, 128-byte requests to L2
+__device__ __forceinline__ uint4 ldg16(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
 }
 
 __device__ __forceinline__ uint4 lds(uint32_t a) {
@@ -259,35 +267,56 @@ __device__ __forceinline__ float fill_q(const T *q, const Params &p, int t, uint
   return up;
 }
 
-// Adds up row r of pieces (m, l, O); a lane takes dims 4 lane, 4 lane + 128, ...
-// List gives the first piece's number, the next one's (-1: none) and a piece's place.
+// Adds up row r of up to 32 pieces (m, l, O) at a time: lane i weighs piece i, then every lane adds dims
+// 4 lane, 4 lane + 128, ... of all pieces, eight loads in flight.  List: how many, and where piece i is.
 template <int DP, class List>
 __device__ __forceinline__ void add_up(const List &list, int r, float4 (&y)[(DP + 127) / 128], float &ref, float &sum) {
   constexpr int ND = (DP + 127) / 128, o_row = DP + 4;
-  const int lane = threadIdx.x % 32;
+  const int lane = threadIdx.x % 32, n = list.count();
   float top = -INFINITY;
-  for (int i = list.first(); i >= 0; i = list.next(i)) top = fmaxf(top, list.load(list.at(i) + kQT * o_row + r));
+  for (int i = lane; i < n; i += 32) top = fmaxf(top, list.load(list.at(i) + kQT * o_row + r));
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
   ref = top == -INFINITY ? 0.f : top;
   sum = 0.f;
 #pragma unroll
   for (int k = 0; k < ND; ++k) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = list.first(); i >= 0; i = list.next(i)) {
-    const float *q = list.at(i);
-    const float f = ex2(list.load(q + kQT * o_row + r) - ref);
-    sum += f * list.load(q + kQT * o_row + kQT + r);
+  for (int base = 0; base < n; base += 32) {
+    float weight = 0.f;
+    const float *mine = nullptr;
+    if (base + lane < n) {
+      mine = list.at(base + lane);
+      const float *q = mine + kQT * o_row + r;
+      weight = ex2(list.load(q) - ref);
+      sum += weight * list.load(q + kQT);
+    }
+    const int here = min(32, n - base);
+    for (int i0 = 0; i0 < here; i0 += 8) {
+      float4 v[8][ND];
 #pragma unroll
-    for (int k = 0; k < ND; ++k) {
-      const int d = 4 * lane + 128 * k;
-      if (d < DP) {
-        const float4 v = list.load(reinterpret_cast<const float4 *>(q + r * o_row + d));
-        y[k].x += f * v.x, y[k].y += f * v.y, y[k].z += f * v.z, y[k].w += f * v.w;
+      for (int i = 0; i < 8; ++i) {
+        const float *q = reinterpret_cast<const float *>(__shfl_sync(~0u, reinterpret_cast<uint64_t>(mine), i0 + i));
+#pragma unroll
+        for (int k = 0; k < ND; ++k) {
+          const int d = 4 * lane + 128 * k;
+          v[i][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i0 + i < here && d < DP) v[i][k] = list.load(reinterpret_cast<const float4 *>(q + r * o_row + d));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = __shfl_sync(~0u, weight, i0 + i);
+        if (i0 + i < here) {
+#pragma unroll
+          for (int k = 0; k < ND; ++k)
+            y[k].x += f * v[i][k].x, y[k].y += f * v[i][k].y, y[k].z += f * v[i][k].z, y[k].w += f * v[i][k].w;
+        }
       }
     }
   }
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
 }
 
-// The pieces of one segment in a block: even numbers in the workspace, odd ones in the warps' slots.
+// The pieces of one segment in a block: even numbers in the workspace, odd ones in the warps' shared memory.
 struct PieceList {
   uint32_t members;
   const float *heads;  // of the block
@@ -295,9 +324,9 @@ struct PieceList {
   int piece, warp_bytes;
   template <class T>
   __device__ T load(const T *q) const { return *q; }  // shared or global memory, of this block's own writing
-  __device__ int first() const { return __ffs(members) - 1; }
-  __device__ int next(int i) const { return i == 31 ? -1 : __ffs(members & (~0u << (i + 1))) - 1; }
-  __device__ const float *at(int i) const {
+  __device__ int count() const { return __popc(members); }
+  __device__ const float *at(int n) const {
+    const int i = __fns(members, 0, n + 1);
     return i % 2 ? reinterpret_cast<const float *>(smem + (i / 2) * warp_bytes) : heads + (i / 2) * piece;
   }
 };
@@ -308,9 +337,8 @@ struct RecordList {
   int piece, from, to;
   template <class T>
   __device__ T load(const T *q) const { return __ldcg(q); }  // written by other blocks
-  __device__ int first() const { return from; }
-  __device__ int next(int b) const { return b < to ? b + 1 : -1; }
-  __device__ const float *at(int b) const { return records + ((int64_t)b * 2 + (b == from)) * piece; }
+  __device__ int count() const { return to - from + 1; }
+  __device__ const float *at(int n) const { return records + ((int64_t)(from + n) * 2 + (n == 0)) * piece; }
 };
 
 template <int MODE, int DP>
@@ -319,7 +347,8 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t s_scan[kMaxWarps];
   __shared__ Cut s_cut[2];
-  __shared__ int64_t s_seg[2 * kMaxWarps], s_end[2 * kMaxWarps], s_seq[2 * kMaxWarps], s_unit[2 * kMaxWarps];
+  // pieces: sequence (-1: none), segment of it, and whether that began before (1) or only ends after (2) this run
+  __shared__ int s_seq[2 * kMaxWarps], s_unit[2 * kMaxWarps], s_open[2 * kMaxWarps];
   __shared__ uint32_t s_masks[2];
   __shared__ int s_last;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
@@ -382,37 +411,36 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
   const int64_t begin = s_cut[0].at, end = s_cut[1].at;
   if (begin >= end) return;
 
-  // ---- this warp's share of it
-  const int64_t wb = begin + (end - begin) * warp / W, we = begin + (end - begin) * (warp + 1) / W;
-  int64_t seq = s_cut[0].seq, seq_begin = s_cut[0].seq_begin;
+  // ---- this warp's share of it; places in the run are counted from its begin from here on
+  const int run = (int)(end - begin);
+  const int wb = (int)((int64_t)run * warp / W), we = (int)((int64_t)run * (warp + 1) / W);
+  int seq = (int)s_cut[0].seq;
+  int64_t seq_begin = s_cut[0].seq_begin - begin;
   Span sp = span_of<C::keys>(p, seq);
-  if (lane < 2) s_seg[2 * warp + lane] = -1;
+  if (lane < 2) s_seq[2 * warp + lane] = -1;
 
-  const int warp_bytes = C::kv + C::q_row * p.q_rows;
+  const int warp_bytes = C::warp_bytes(p.q_rows);
   uint8_t *own = smem + warp * warp_bytes;
-  const uint32_t slots = (uint32_t)__cvta_generic_to_shared(own) + lane * 16;
   // query row g in fragment order; lanes beyond the tile's rows repeat its last one, their results go nowhere
-  const uint32_t sq = (uint32_t)__cvta_generic_to_shared(own) + C::kv + min(g, p.q_rows - 1) * 64 + t * 16;
+  const uint32_t sq = (uint32_t)__cvta_generic_to_shared(own) + min(g, p.q_rows - 1) * 64 + t * 16;
   const int q_step = p.q_rows * 64;
-  const bool paged16 = ps % 16 == 0;
+  const bool paged16 = ps % 16 == 0, full_dim = D == DP;
   const uint8_t *kbase = static_cast<const uint8_t *>(p.pool.k), *vbase = static_cast<const uint8_t *>(p.pool.v);
-  const int64_t kslot = p.pool.k_stride[2] * C::es, vslot = p.pool.v_stride[2] * C::es;
-  const int64_t kpage = p.pool.k_stride[0] * C::es, vpage = p.pool.v_stride[0] * C::es;
 
-  for (int64_t at = wb; at < we;) {
+  for (int at = wb; at < we;) {
     while (at >= seq_begin + sp.steps * units) {  // next sequence with keys
       seq_begin += sp.steps * units;
       sp = span_of<C::keys>(p, ++seq);
     }
-    const int64_t off = at - seq_begin, unit = off / sp.steps;
-    const int step0 = (int)(off - unit * sp.steps);
-    const int h = (int)(unit / p.qtiles), qt = (int)(unit % p.qtiles);
-    const int64_t seg_begin = seq_begin + unit * sp.steps, seg_end = seg_begin + sp.steps;
-    const int n = (int)((seg_end < we ? seg_end : we) - at);
+    const int64_t off = at - seq_begin;
+    const int unit = (int)(off / sp.steps), step0 = (int)(off - (int64_t)unit * sp.steps);
+    const int h = unit / p.qtiles, qt = unit - h * p.qtiles;
+    const int n = min(sp.steps - step0, we - at);
+    const bool whole = step0 == 0 && n == sp.steps;
     const int rows = min(kQT, p.group - qt * kQT), head0 = h * p.group + qt * kQT;
     const int32_t *table = p.a.page_table + seq * p.a.table_stride;
     const int key0 = sp.start + step0 * C::keys;
-    const uint8_t *kh = kbase + h * p.pool.k_stride[1] * C::es, *vh = vbase + h * p.pool.v_stride[1] * C::es;
+    const uint8_t *kh = kbase + h * p.k_head, *vh = vbase + h * p.v_head;
 
     // ---- places of a step's keys: a page entry per 16 keys, or one per key
     constexpr int NS = C::keys / C::sub;
@@ -450,45 +478,46 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
       if (bad) serve::set_status(p.status, 8);
       return mask;
     };
-    // the row of key k8 + k of a step; k8 a constant multiple of 8, k below 8
-    auto row_of = [&](const uint8_t *base, int64_t page, int64_t slot, int key, int k8, int k) -> const uint8_t * {
-      if (paged16) {
-        const int first = key + k8 / 16 * 16;
-        return base + entry[k8 / 16] * page + (first - page_of(p, first) * ps + k8 % 16 + k) * slot;
+    // Loads this lane's pieces of the keys of the step at `key`: of K, piece t + 4j of key 8 nt + g; of V, piece
+    // g + 8j of keys 8 nt + 2t + (0, 1).  Absent keys and pieces beyond head_dim are zeros.
+    uint4 kf[C::NT][C::KJ], vf[2 * C::NT][C::VJ];
+    auto load = [&](auto &f, const uint8_t *base, int64_t page, int64_t slot, int key, uint32_t mask, bool is_k) {
+      constexpr int rows = sizeof(f) / sizeof(f[0]), J = sizeof(f[0]) / sizeof(f[0][0]);
+      const int lane_row = is_k ? g : 2 * t, first_piece = is_k ? t : g, piece_step = is_k ? 4 : 8;
+      const bool full = full_dim && mask == (uint32_t)((1ull << C::keys) - 1);
+      const uint8_t *block = base;
+#pragma unroll
+      for (int r = 0; r < rows; ++r) {
+        const int k8 = is_k ? r * 8 : r / 2 * 8, k = is_k ? g : 2 * t + r % 2;  // key k8 + k
+        const uint8_t *src;
+        if (paged16) {
+          const int first = key + k8 / 16 * 16;
+          if (k8 % 16 == 0 && (is_k || r % 2 == 0))
+            block = base + entry[k8 / 16] * page + (first - page_of(p, first) * ps + lane_row) * slot + first_piece * 16;
+          src = block + (k8 % 16 + (is_k ? 0 : r % 2)) * slot;
+        } else {
+          const int e = __shfl_sync(~0u, entry[0], k8 + k), kk = key + k8 + k;
+          src = base + e * page + (kk - page_of(p, kk) * ps) * slot + first_piece * 16;
+        }
+        if (full) {
+#pragma unroll
+          for (int j = 0; j < J; ++j) f[r][j] = ldg16(src + j * piece_step * 16);
+        } else {
+          const bool ok = mask >> (k8 + k) & 1;
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            f[r][j] = make_uint4(0, 0, 0, 0);
+            if (ok && (first_piece + piece_step * j) * C::epc < D) f[r][j] = ldg16(src + j * piece_step * 16);
+          }
+        }
       }
-      const int e = __shfl_sync(~0u, entry[0], k8 + k), kk = key + k8 + k;
-      return base + e * page + (kk - page_of(p, kk) * ps) * slot;
     };
-    auto copy_k = [&](int key, uint32_t mask) {
-#pragma unroll
-      for (int nt = 0; nt < C::NT; ++nt) {
-        const int k = nt * 8 + g;
-        const uint8_t *src = row_of(kh, kpage, kslot, key, nt * 8, g) + t * 16;
-        const bool ok = mask >> k & 1;
-        if (!ok) src = kbase;
-#pragma unroll
-        for (int j = 0; j < C::KJ; ++j)
-          copy16(slots + (nt * C::KJ + j) * 512, src + j * 64, ok && (t + 4 * j) * C::epc < D);
-      }
-    };
-    auto copy_v = [&](int key, uint32_t mask) {
-#pragma unroll
-      for (int kk = 0; kk < 2 * C::NT; ++kk) {
-        const int k = (kk / 2) * 8 + 2 * t + kk % 2;
-        const uint8_t *src = row_of(vh, vpage, vslot, key, kk / 2 * 8, 2 * t + kk % 2) + g * 16;
-        const bool ok = mask >> k & 1;
-        if (!ok) src = vbase;
-#pragma unroll
-        for (int j = 0; j < C::VJ; ++j)
-          copy16(slots + (C::k_slots + kk * C::VJ + j) * 512, src + j * 128, ok && (g + 8 * j) * C::epc < D);
-      }
-    };
+    auto load_k = [&](int key, uint32_t mask) { load(kf, kh, p.k_page, p.k_slot, key, mask, true); };
+    auto load_v = [&](int key, uint32_t mask) { load(vf, vh, p.v_page, p.v_slot, key, mask, false); };
     look_up(key0);
     uint32_t mask = present_of(key0);
-    copy_k(key0, mask);
-    asm volatile("cp.async.commit_group;");
-    copy_v(key0, mask);
-    asm volatile("cp.async.commit_group;");
+    load_k(key0, mask);
+    load_v(key0, mask);
 
     // ---- the query tile, split into parts, in fragment order
     const int64_t q0 = seq * p.a.q.stride[0] + (head0 + min(g, rows - 1)) * p.a.q.stride[1];
@@ -514,7 +543,6 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
     if (n > 1) look_up(key0 + C::keys);
     for (int i = 0; i < n; ++i) {
       const int next = key0 + (i + 1) * C::keys;
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
       float s[C::NT][2][4] = {};
 #pragma unroll
       for (int j = 0; j < C::KJ; ++j) {
@@ -523,7 +551,7 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
         for (int part = 0; part < C::parts; ++part) q[part] = lds(sq + (j * C::parts + part) * q_step);
 #pragma unroll
         for (int nt = 0; nt < C::NT; ++nt) {
-          const uint4 k = lds(slots + (nt * C::KJ + j) * 512);
+          const uint4 k = kf[nt][j];
           if (C::f32) {
             const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
             const uint32_t qh[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
@@ -549,9 +577,8 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
       const uint32_t now = mask;
       if (i + 1 < n) {
         mask = present_of(next);
-        copy_k(next, mask);
+        if (C::ahead) load_k(next, mask);
       }
-      asm volatile("cp.async.commit_group;");
       // running maximum and sum; a lane has query g and keys 2t, 2t+1 of every 8
       float x[C::NT][2], top = -INFINITY;
 #pragma unroll
@@ -599,13 +626,12 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
           }
         }
       }
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
 #pragma unroll
       for (int j = 0; j < C::VJ; ++j) {
         uint32_t v[2 * C::NT][4];
 #pragma unroll
         for (int kk = 0; kk < 2 * C::NT; ++kk) {
-          const uint4 w = lds(slots + (C::k_slots + kk * C::VJ + j) * 512);
+          const uint4 w = vf[kk][j];
           v[kk][0] = w.x, v[kk][1] = w.y, v[kk][2] = w.z, v[kk][3] = w.w;
         }
 #pragma unroll
@@ -632,16 +658,15 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
         }
       }
       if (i + 1 < n) {
-        copy_v(next, mask);
+        if (!C::ahead) load_k(next, mask);
+        load_v(next, mask);
         if (i + 2 < n) look_up(next + C::keys);
       }
-      asm volatile("cp.async.commit_group;");
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     l += __shfl_xor_sync(~0u, l, 1);
     l += __shfl_xor_sync(~0u, l, 2);
-    __syncwarp();  // every lane has read its last slots
-    if (at == seg_begin && at + n == seg_end) {
+    __syncwarp();  // every lane is done with the query tile
+    if (whole) {
       if (g < rows) {
         const float scale = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -659,7 +684,7 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
         if (p.a.lse && t == 0) p.a.lse[seq * p.q_heads + head0 + g] = lse_of(m == -INFINITY ? 0.f : m, l);
       }
     } else {
-      // the last piece of a run stays in the warp's slots, an earlier one goes to the workspace
+      // the last piece of a run stays in shared memory, an earlier one goes to the workspace
       const int tail = at + n == we;
       float *to = tail ? reinterpret_cast<float *>(own) : p.heads + ((int64_t)blockIdx.x * W + warp) * C::piece;
 #pragma unroll
@@ -679,7 +704,7 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
       }
       if (lane == 0) {
         const int i = 2 * warp + tail;
-        s_seg[i] = seg_begin, s_end[i] = seg_end, s_seq[i] = seq, s_unit[i] = unit;
+        s_seq[i] = seq, s_unit[i] = unit, s_open[i] = at - step0 < 0 ? 1 : at - step0 + sp.steps > run ? 2 : 0;
       }
     }
     at += n;
@@ -688,9 +713,10 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
   // ---- the block's pieces, one warp per segment and row
   __syncthreads();
   if (warp == 0) {
-    const bool has = lane < 2 * W && s_seg[lane] >= 0;
+    const bool has = lane < 2 * W && s_seq[lane] >= 0;
     const uint32_t valid = __ballot_sync(~0u, has), earlier = valid & ((1u << lane) - 1);
-    const bool leads = has && (!earlier || s_seg[31 - __clz(earlier)] != s_seg[lane]);
+    const int prev = 31 - __clz(earlier);
+    const bool leads = has && (!earlier || s_seq[prev] != s_seq[lane] || s_unit[prev] != s_unit[lane]);
     const uint32_t leaders = __ballot_sync(~0u, leads);
     if (lane == 0) s_masks[0] = valid, s_masks[1] = leaders;
   }
@@ -715,17 +741,16 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
     const int lead = __ffs(leaders) - 1;
     leaders &= leaders - 1;
     const uint32_t members = valid & ~((1u << lead) - 1) & (leaders ? (1u << (__ffs(leaders) - 1)) - 1 : ~0u);
-    const int64_t unit = s_unit[lead];
-    const int qt = (int)(unit % p.qtiles), head = (int)(unit / p.qtiles) * p.group + qt * kQT + r;
+    const int unit = s_unit[lead], qt = unit % p.qtiles, head = unit / p.qtiles * p.group + qt * kQT + r;
     if (qt * kQT + r >= p.group) continue;
     float4 y[ND];
     float ref, sum;
     add_up<DP>(PieceList{members, p.heads + (int64_t)blockIdx.x * W * C::piece, smem, C::piece, warp_bytes}, r, y, ref,
                sum);
-    if (s_seg[lead] >= begin && s_end[lead] <= end) {
+    if (s_open[lead] == 0) {
       write_row(s_seq[lead], head, y, ref, sum);
     } else {
-      float *rec = p.records + ((int64_t)blockIdx.x * 2 + (s_seg[lead] >= begin)) * C::piece;
+      float *rec = p.records + ((int64_t)blockIdx.x * 2 + s_open[lead] - 1) * C::piece;
 #pragma unroll
       for (int k = 0; k < ND; ++k)
         if (4 * lane + 128 * k < DP) *reinterpret_cast<float4 *>(rec + r * C::o_row + 4 * lane + 128 * k) = y[k];
