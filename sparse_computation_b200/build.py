@@ -27,10 +27,12 @@ CXXFLAGS = ["-O3", "-std=c++17", "-fPIC", "-pthread", "-Wall", "-Wno-unused-func
 
 HOST_SOURCES = ["sc_host.cpp"]
 # (source, extra flags, object name): sc_inst.cu is compiled once per
-# (kernel_m, wide|narrow); the slowest units are listed first.
+# (kernel_m, wide|narrow), sc_attn_inst.cu once per operand mode; the slowest
+# units are listed first.
 CUDA_SOURCES = [("sc_plan.cu", [], "sc_plan.cu.o"), ("sc_dense.cu", [], "sc_dense.cu.o"),
                 ("sc_noalloc.cu", [], "sc_noalloc.cu.o"), ("sc_serve.cu", [], "sc_serve.cu.o"),
                 ("sc_adapters.cu", [], "sc_adapters.cu.o"), ("sc_attn.cu", [], "sc_attn.cu.o")] + [
+    ("sc_attn_inst.cu", [f"-DSC_ATTN_MODE={m}"], f"sc_attn_inst_{m}.cu.o") for m in range(6)] + [
     ("sc_inst.cu", [f"-DSC_KM={km}", f"-DSC_PART={part}"], f"sc_inst_km{km}_{'wn'[part]}.cu.o")
     for km in (4, 6, 5, 3, 2, 1) for part in (0, 1)]
 

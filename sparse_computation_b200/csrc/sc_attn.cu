@@ -8,41 +8,6 @@
 using namespace sc::serve;
 using namespace sc::attn;
 
-namespace {
-
-// One instantiation of the kernel and what its launch needs.
-struct Variant {
-  void (*kernel)(Params);
-  int warps, smem, keys, piece;
-};
-
-// As many warps as registers (Cfg::max_warps) and shared memory (a query tile
-// or a piece each) allow.
-template <int MODE, int DP>
-Variant variant(int q_rows, int smem_limit) {
-  using C = Cfg<MODE, DP>;
-  const int per_warp = C::warp_bytes(q_rows);
-  Variant v{attend_kernel<MODE, DP>, 0, 0, C::keys, C::piece};
-  cudaFuncAttributes attr;
-  cuda_check(cudaFuncGetAttributes(&attr, v.kernel), "kernel attributes");
-  v.warps = std::min(C::max_warps, (smem_limit - (int)attr.sharedSizeBytes) / per_warp);
-  v.smem = v.warps * per_warp;
-  require(v.warps > 0, SC_ERR_CUDA, "the attention kernel does not fit this GPU");
-  cuda_check(cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  smem_limit - (int)attr.sharedSizeBytes),
-             "set shared memory size");
-  return v;
-}
-
-template <int MODE>
-Variant variant_for(int64_t head_dim, int q_rows, int smem_limit) {
-  return head_dim <= 64    ? variant<MODE, 64>(q_rows, smem_limit)
-         : head_dim <= 128 ? variant<MODE, 128>(q_rows, smem_limit)
-                           : variant<MODE, 256>(q_rows, smem_limit);
-}
-
-}  // namespace
-
 struct sc_attn {
   sc_kv_pool pool;
   int device = 0;
@@ -51,7 +16,7 @@ struct sc_attn {
   int qtiles = 0, q_rows = 0, sms = 0;
   uint32_t page_mul = 0, page_shift = 0;
   Variant same, other;  // q of the cache's type; q of another type
-  DeviceBlock mem;      // status | arrivals | pieces | records
+  DeviceBlock mem;      // status | 1 KB of zeros | arrivals | pieces | records
   int *status = nullptr, *arrivals = nullptr;
   float *heads = nullptr, *records = nullptr;
 };
@@ -88,6 +53,10 @@ int sc_attn_create(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, 
       p->page_shift = bits - 1;
       break;
     }
+  const int64_t unit = 16 / type_bytes(pool.type);
+  for (const int64_t *st : {pool.k_stride, pool.v_stride})
+    require(((pool.num_pages - 1) * st[0] + (pool.page_size - 1) * st[2]) / unit <= UINT32_MAX, SC_ERR_UNSUPPORTED,
+            "a cache pool of 64 GB or more");
   DeviceGuard dg(p->device);
   int limit = 0;
   cuda_check(cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, p->device), "device attribute");
@@ -99,15 +68,17 @@ int sc_attn_create(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, 
     p->other = variant_for<kF16Wide>(pool.head_dim, p->q_rows, limit);
   } else {
     p->same = variant_for<kBF16>(pool.head_dim, p->q_rows, limit);
-    p->other = variant_for<kBF16Wide>(pool.head_dim, p->q_rows, limit);
+    // three parts of up to four query heads share an instruction's 16 rows
+    p->other = p->q_rows <= 4 ? variant_for<kBF16Wide4>(pool.head_dim, p->q_rows, limit)
+                              : variant_for<kBF16Wide>(pool.head_dim, p->q_rows, limit);
   }
-  const size_t words = 64 + ((size_t)segments + 63) / 64 * 64, piece = (size_t)p->same.piece;
+  const size_t words = 64 + 256 + ((size_t)segments + 63) / 64 * 64, piece = (size_t)p->same.piece;
   const size_t heads = (size_t)p->sms * std::max(p->same.warps, p->other.warps) * piece;
   p->mem.alloc(p->device, (words + heads + (size_t)p->sms * 2 * piece) * 4, "allocate attention workspace");
   cuda_check(cudaMemset(p->mem.p, 0, words * 4), "clear attention workspace");
   cuda_check(cudaDeviceSynchronize(), "device synchronize");
   p->status = static_cast<int *>(p->mem.p);
-  p->arrivals = p->status + 64;
+  p->arrivals = p->status + 64 + 256;
   p->heads = reinterpret_cast<float *>(p->status + words);
   p->records = p->heads + heads;
   *out = p.release();
@@ -132,21 +103,24 @@ int sc_attn_decode(sc_attn *p, const sc_attn_args *a, void *stream) {
   require(a->q.ptr && a->out.ptr && a->page_table && a->seq_lens, SC_ERR_ARG,
           "null q, out, page table or lengths");
   require(a->table_cols >= 0 && a->table_stride >= 0, SC_ERR_ARG, "bad page table sizes");
-  const int64_t e = type_bytes(a->type), ce = type_bytes(p->pool.type);
-  const int q_vec = a->q.stride[2] == 1 && a->q.stride[1] * e % 16 == 0 && a->q.stride[0] * e % 16 == 0 &&
-                    reinterpret_cast<uintptr_t>(a->q.ptr) % 16 == 0 && p->pool.head_dim % 8 == 0;
   const Variant &v = a->type == p->pool.type ? p->same : p->other;
-  Params k{*a, p->pool, (int)p->q_heads, (int)(p->q_heads / p->pool.kv_heads), p->qtiles, p->q_rows, v.warps,
-           p->page_mul, p->page_shift, q_vec, p->pool.k_stride[0] * ce, p->pool.k_stride[1] * ce, p->pool.k_stride[2] * ce,
-           p->pool.v_stride[0] * ce, p->pool.v_stride[1] * ce, p->pool.v_stride[2] * ce,
-           (float)(p->scale * 1.4426950408889634), p->window, p->status, p->arrivals,
-           p->heads, p->records};
+  const int64_t unit = 16 / type_bytes(p->pool.type);  // elements in 16 bytes
+  const int64_t qe = type_bytes(a->type);
+  const int q_vec = a->q.stride[2] == 1 && a->q.stride[1] * qe % 16 == 0 && a->q.stride[0] * qe % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(a->q.ptr) % 16 == 0 && p->pool.head_dim * qe % 16 == 0;
+  Params k{*a, p->pool, (int)p->q_heads, (int)(p->q_heads / p->pool.kv_heads), p->qtiles, p->q_rows, v.warps, q_vec,
+           p->page_mul, p->page_shift, (uint32_t)(p->pool.k_stride[0] / unit), (uint32_t)(p->pool.k_stride[2] / unit),
+           (uint32_t)(p->pool.v_stride[0] / unit), (uint32_t)(p->pool.v_stride[2] / unit),
+           (float)(p->scale * 1.4426950408889634), p->window, p->status,
+           reinterpret_cast<const uint8_t *>(p->status + 64), p->arrivals, p->heads, p->records};
   // the most steps that these lengths can have; the true number is known on the device only
   int64_t keys = std::min<int64_t>(a->table_cols, INT32_MAX / p->pool.page_size) * p->pool.page_size;
   if (p->window) keys = std::min(keys, p->window + 15);
-  const int64_t steps = std::max<int64_t>(1, (keys + v.keys - 1) / v.keys) * a->seqs * p->pool.kv_heads * p->qtiles;
-  const int64_t blocks = std::min<int64_t>((steps + v.warps - 1) / v.warps, p->sms);
-  require(steps / blocks < INT32_MAX / 2, SC_ERR_UNSUPPORTED, "the table names more keys than one call can take");
+  const int64_t per_seq = std::max<int64_t>(1, (keys + v.keys - 1) / v.keys) + kSwitch, units = p->pool.kv_heads * p->qtiles;
+  // places are counted in 32 bits, and a block's run may end one run beyond the last
+  require(per_seq * a->seqs * units < INT32_MAX / 2, SC_ERR_UNSUPPORTED,
+          "the page table names more keys than one call can take");
+  const int64_t blocks = std::min<int64_t>((per_seq * a->seqs * units + v.warps - 1) / v.warps, p->sms);
   DeviceGuard dg(p->device);
   v.kernel<<<(unsigned)blocks, v.warps * 32, v.smem, static_cast<cudaStream_t>(stream)>>>(k);
   cuda_check(cudaGetLastError(), "launch decode attention");
