@@ -1,6 +1,8 @@
 // Cache append with the rotary rotation.
+#include <algorithm>
 #include <cmath>
 #include <memory>
+#include <type_traits>
 
 #include "sc_serve.h"
 
@@ -16,6 +18,9 @@ struct AppendParams {
   sc_kv_append_args a;
   sc_kv_pool pool;
   int *status;
+  uint32_t page_mul, page_shift;    // divider by the page size
+  uint32_t pairs_mul, pairs_shift;  // divider by the pairs of a head
+  int tile_bits, parts;
 };
 
 // The cache place of token t: page and slot, or page -1 when it is skipped.
@@ -26,7 +31,7 @@ __device__ __forceinline__ void token_place(const AppendParams &p, int64_t t, in
   pos = a.positions[t];
   if (pos < 0) return;
   const int64_t seq = a.seq_ids ? a.seq_ids[t] : t;
-  const int col = pos / (int)p.pool.page_size;
+  const int col = p.page_mul ? (int)(__umulhi((uint32_t)pos, p.page_mul) >> p.page_shift) : pos;
   if (seq < 0 || seq >= a.seqs || col >= a.table_cols) {
     set_status(p.status, 8);
     return;
@@ -44,10 +49,10 @@ __device__ __forceinline__ void token_place(const AppendParams &p, int64_t t, in
   slot = pos - col * (int)p.pool.page_size;
 }
 
-// One thread per pair of dims that rotate together (or two neighbouring ones
-// that do not) of one head of one token.
+// Any strides: one thread per pair of dims that rotate together (or two
+// neighbouring ones that do not) of one head of one token.
 template <class T, class C>
-__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(256) append_any_kernel(const AppendParams p) {
   const sc_kv_append_args &a = p.a;
   const int pairs = (int)p.pool.head_dim / 2;
   const int hk = (int)p.pool.kv_heads, hq = a.q.ptr ? (int)a.q_heads : 0;
@@ -93,6 +98,250 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
     y[d0] = from_f32<C>(u);
     y[d1] = from_f32<C>(w);
   }
+}
+
+// Eight neighbouring elements, as they lie.
+template <class T>
+struct Eight {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(p)[i];
+  }
+  __device__ __forceinline__ void store(T *p) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(p)[i] = w[i];
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const T *v = reinterpret_cast<const T *>(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(v[i]);
+  }
+  __device__ __forceinline__ void set(const float (&x)[8]) {
+    T *v = reinterpret_cast<T *>(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = from_f32<T>(x[i]);
+  }
+};
+
+// n / by for n below 2^31, as umulhi(n, mul) >> shift (mul 0: by is 1).
+struct Divider {
+  uint32_t by = 1, mul = 0, shift = 0;
+  Divider() = default;
+  explicit Divider(int64_t d) : by((uint32_t)d) {
+    for (int bits = 1; d > 1; ++bits)
+      if (((int64_t)1 << bits) >= d) {
+        mul = (uint32_t)((((uint64_t)1 << (31 + bits)) + d - 1) / d);
+        shift = bits - 1;
+        return;
+      }
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return mul ? __umulhi(n, mul) >> shift : n; }
+};
+
+// Token-major activations (the heads of a token contiguous): a warp takes a
+// token, or 1/p.parts of it, so that position, page and rotation row are its
+// own scalars, and walks the heads in jobs of eight dims (with their eight
+// partners in the half style), BATCH of them in flight.  Bound by memory, but
+// at 16 bits the instructions of a job count as much: index computations of
+// one flat job list over all tokens took 20 us for 4099 tokens, against TODO.
+struct RowJobs {
+  Divider jobs;  // of a head
+  int half;      // distance of partners, 0: none
+};
+
+template <class T, class C, int BATCH, bool POOL>
+__device__ __forceinline__ void walk_heads(const T *src, C *dst, int64_t dst_head, const RowJobs &r, int heads, int rotary,
+                                           const float *cos, const float *sin, bool rope4, bool zero, int first, int step) {
+  const int n = heads * (int)r.jobs.by, D = (int)r.jobs.by * 8 + r.half;
+  for (int j0 = first; j0 < n; j0 += BATCH * step) {
+    Eight<T> u[BATCH], w[BATCH];
+    int d[BATCH], head[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int j = j0 + i * step;
+      head[i] = (int)r.jobs(j);
+      d[i] = (j - head[i] * (int)r.jobs.by) * 8;
+      if (d[i] >= r.half) d[i] += r.half;  // the partners' eights go with the first ones
+      if (j < n) {
+        u[i].load(src + head[i] * D + d[i]);
+        if (d[i] < r.half) w[i].load(src + head[i] * D + d[i] + r.half);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      if (j0 + i * step >= n) break;
+      C *y = dst + (POOL ? head[i] * dst_head : head[i] * D) + d[i];
+      const bool two = d[i] < r.half;
+      if (std::is_same<T, C>::value && d[i] >= rotary && !zero) {  // the bits move as they are
+        u[i].store(reinterpret_cast<T *>(y));
+        if (two) w[i].store(reinterpret_cast<T *>(y + r.half));
+        continue;
+      }
+      float x[8], z[8] = {};
+      u[i].get(x);
+      if (two) w[i].get(z);
+      if (d[i] < rotary) {
+        const float *cp = cos + (r.half ? d[i] : d[i] / 2), *sp = sin + (r.half ? d[i] : d[i] / 2);
+        float c[8], s[8];
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+          if (e == 0 || r.half) {
+            if (rope4) {
+              *reinterpret_cast<float4 *>(c + e) = *reinterpret_cast<const float4 *>(cp + e);
+              *reinterpret_cast<float4 *>(s + e) = *reinterpret_cast<const float4 *>(sp + e);
+            } else {
+#pragma unroll
+              for (int f = e; f < e + 4; ++f) c[f] = cp[f], s[f] = sp[f];
+            }
+          }
+        if (r.half) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float v = x[e] * c[e] - z[e] * s[e];
+            z[e] = z[e] * c[e] + x[e] * s[e];
+            x[e] = v;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float v = x[e] * c[e / 2] - x[e + 1] * s[e / 2];
+            x[e + 1] = x[e + 1] * c[e / 2] + x[e] * s[e / 2];
+            x[e] = v;
+          }
+        }
+      }
+      if (zero)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = z[e] = 0.f;
+      Eight<C> o;
+      o.set(x);
+      o.store(y);
+      if (two) {
+        o.set(z);
+        o.store(y + r.half);
+      }
+    }
+  }
+}
+
+template <class T, class C>
+__global__ void __launch_bounds__(128) append_rows_kernel(const __grid_constant__ AppendParams p, const __grid_constant__ RowJobs turned,
+                                                          const __grid_constant__ RowJobs plain, int rope4) {
+  constexpr int B = sizeof(T) == 4 ? 2 : 4;
+  const sc_kv_append_args &a = p.a;
+  const int64_t t = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32;
+  if (t >= a.tokens) return;
+  int pos, page, slot;
+  token_place(p, t, pos, page, slot);
+  const int first = blockIdx.y * 32 + threadIdx.x % 32, step = 32 * p.parts;
+  const int rotary = a.cos && page >= 0 ? (int)a.rotary : 0, hk = (int)p.pool.kv_heads;
+  const float *cos = a.cos + pos * a.rope_stride, *sin = a.sin + pos * a.rope_stride;
+  if (page >= 0) {
+    walk_heads<T, C, B, true>(static_cast<const T *>(a.v.ptr) + t * a.v.stride[0],
+                              static_cast<C *>(p.pool.v) + page * p.pool.v_stride[0] + slot * p.pool.v_stride[2],
+                              p.pool.v_stride[1], plain, hk, 0, cos, sin, false, false, first, step);
+    walk_heads<T, C, B, true>(static_cast<const T *>(a.k.ptr) + t * a.k.stride[0],
+                              static_cast<C *>(p.pool.k) + page * p.pool.k_stride[0] + slot * p.pool.k_stride[2],
+                              p.pool.k_stride[1], turned, hk, rotary, cos, sin, rope4, false, first, step);
+  }
+  if (a.q.ptr)
+    walk_heads<T, T, B, false>(static_cast<const T *>(a.q.ptr) + t * a.q.stride[0],
+                               static_cast<T *>(a.q_out.ptr) + t * a.q_out.stride[0], 0, turned, (int)a.q_heads, rotary, cos,
+                               sin, rope4, page < 0, first, step);
+}
+
+// Feature-major activations, as a product leaves them (tokens contiguous): a
+// block takes one head of 2^p.tile_bits tokens, reads it along the tokens,
+// turns it in shared memory and writes it along the dims, two to a thread.
+template <class T, class C>
+__global__ void __launch_bounds__(256) append_columns_kernel(const __grid_constant__ AppendParams p) {
+  const sc_kv_append_args &a = p.a;
+  __shared__ float tile[kMaxHeadDim * 33];
+  __shared__ int s_pos[32], s_slot[32], s_page[32];
+  const int hk = (int)p.pool.kv_heads, hq = a.q.ptr ? (int)a.q_heads : 0, D = (int)p.pool.head_dim;
+  const int TT = 1 << p.tile_bits, width = TT + 1;
+  const int64_t t0 = (int64_t)blockIdx.y << p.tile_bits;
+  const int here = (int)min((int64_t)TT, a.tokens - t0);
+  int head = blockIdx.x;
+  const bool is_q = head < hq, is_v = head >= hq + hk;
+  const sc_rows &src = is_q ? a.q : is_v ? a.v : a.k;
+  if (!is_q) head -= is_v ? hq + hk : hq;
+  const T *x = static_cast<const T *>(src.ptr) + t0 + head * src.stride[1];
+  // the first loads are on their way while the places, two dependent loads, are worked out
+  constexpr int B = 16;
+  auto load = [&](int i0, T (&v)[B]) {
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      const int i = i0 + 256 * k, d = i >> p.tile_bits, t = i & (TT - 1);
+      if (d < D && t < here) v[k] = x[d * src.stride[2] + t];
+    }
+  };
+  auto keep = [&](int i0, const T (&v)[B]) {
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      const int i = i0 + 256 * k, d = i >> p.tile_bits, t = i & (TT - 1);
+      if (d < D && t < here) tile[d * width + t] = to_f32(v[k]);
+    }
+  };
+  T v[B];
+  load(threadIdx.x, v);
+  if ((int)threadIdx.x < here) {
+    int pos, page, slot;
+    token_place(p, t0 + threadIdx.x, pos, page, slot);
+    s_pos[threadIdx.x] = pos, s_page[threadIdx.x] = page, s_slot[threadIdx.x] = slot;
+  }
+  keep(threadIdx.x, v);
+#pragma unroll 1
+  for (int i0 = threadIdx.x + B * 256; i0 < D << p.tile_bits; i0 += B * 256) {
+    load(i0, v);
+    keep(i0, v);
+  }
+  __syncthreads();
+  const int rotary = a.cos && !is_v ? (int)a.rotary : 0, half = rotary / 2, pairs = D / 2;
+  const bool halves = !a.interleaved;
+  for (int i = threadIdx.x; i < pairs * here; i += 256) {
+    const int t = p.pairs_mul ? (int)(__umulhi(i, p.pairs_mul) >> p.pairs_shift) : i, d = 2 * (i - t * pairs);
+    const int page = s_page[t], pos = s_pos[t];
+    if (page < 0 && !is_q) continue;
+    float u = tile[d * width + t], w = tile[(d + 1) * width + t];
+    if (page < 0) {
+      u = w = 0.f;
+    } else if (d < rotary) {
+      const float *c = a.cos + pos * a.rope_stride, *s = a.sin + pos * a.rope_stride;
+      if (halves) {  // half is even: both dims lie on one side
+        const bool upper = d >= half;
+        const int i0 = upper ? d - half : d, other = upper ? d - half : d + half;
+        const float sign = upper ? 1.f : -1.f;
+        u = u * c[i0] + sign * (tile[other * width + t] * s[i0]);
+        w = w * c[i0 + 1] + sign * (tile[(other + 1) * width + t] * s[i0 + 1]);
+      } else {
+        const float ci = c[d / 2], si = s[d / 2], ru = u * ci - w * si;
+        w = w * ci + u * si;
+        u = ru;
+      }
+    }
+    auto put = [&](auto *y) {
+      using E = std::remove_reference_t<decltype(*y)>;
+      struct alignas(2 * sizeof(E)) Two {
+        E a, b;
+      };
+      *reinterpret_cast<Two *>(y) = Two{from_f32<E>(u), from_f32<E>(w)};
+    };
+    if (is_q) {
+      put(static_cast<T *>(a.q_out.ptr) + (t0 + t) * a.q_out.stride[0] + head * a.q_out.stride[1] + d);
+    } else {
+      const int64_t *st = is_v ? p.pool.v_stride : p.pool.k_stride;
+      put(static_cast<C *>(is_v ? p.pool.v : p.pool.k) + page * st[0] + head * st[1] + s_slot[t] * st[2] + d);
+    }
+  }
+}
+
+// Whether rows of `type` are contiguous along the dims with every `elems`-th element aligned to a vector of that many.
+bool along_dims(const sc_rows &r, int64_t tokens, int64_t type, int64_t elems) {
+  const int64_t e = type_bytes(type), n = elems * e < 16 ? elems * e : 16;
+  return r.stride[2] == 1 && (tokens == 1 || r.stride[0] * e % n == 0) && r.stride[1] * e % n == 0 &&
+         reinterpret_cast<uintptr_t>(r.ptr) % n == 0;
 }
 
 template <class F>
@@ -173,13 +422,48 @@ int sc_kv_append(sc_kv_cache *c, const sc_kv_append_args *a, void *stream) {
   if (a->cos)
     require(a->rotary > 0 && a->rotary % 2 == 0 && a->rotary <= c->pool.head_dim && a->rope_rows > 0, SC_ERR_ARG,
             "rotary must be even and at most head_dim");
-  AppendParams p{*a, c->pool, static_cast<int *>(c->status.p)};
+  const Divider by_page(c->pool.page_size);
+  AppendParams p{*a, c->pool, static_cast<int *>(c->status.p), by_page.mul, by_page.shift, 0, 0, 0, 0};
   DeviceGuard dg(c->device);
-  const int64_t n = a->tokens * ((a->q.ptr ? a->q_heads : 0) + 2 * c->pool.kv_heads) * (c->pool.head_dim / 2);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool q = a->q.ptr != nullptr, rotates = a->cos != nullptr, halves = rotates && !a->interleaved;
+  const int64_t D = c->pool.head_dim, heads = (q ? a->q_heads : 0) + 2 * c->pool.kv_heads;
+  const int64_t half = rotates ? a->rotary / 2 : 0;
+  auto packed = [&](const sc_rows &r, int64_t h) { return h == 1 || r.stride[1] == D; };
+  // Token-major rows with packed heads move in eights, feature-major ones through shared memory; what fits neither
+  // (odd strides, a rotation that splits an eight) goes element by element.
+  const bool rows = D % 8 == 0 && half % 8 == 0 && heads <= 65535 && packed(a->k, c->pool.kv_heads) && packed(a->v, c->pool.kv_heads) &&
+                    along_dims(a->k, a->tokens, a->type, 8) && along_dims(a->v, a->tokens, a->type, 8) &&
+                    (!q || (packed(a->q, a->q_heads) && packed(a->q_out, a->q_heads) &&
+                            along_dims(a->q, a->tokens, a->type, 8) && along_dims(a->q_out, a->tokens, a->type, 8)));
+  const bool columns = half % 2 == 0 && (!q || (a->q.stride[0] == 1 && along_dims(a->q_out, a->tokens, a->type, 2))) &&
+                       a->k.stride[0] == 1 && a->v.stride[0] == 1 && heads <= 65535;
+  const int64_t n = a->tokens * heads * (D / 2);
   require((n + 255) / 256 <= INT32_MAX, SC_ERR_UNSUPPORTED, "too many rows in one call");
   with_types(a->type, c->pool.type, [&](auto t, auto e) {
-    append_kernel<decltype(t), decltype(e)>
-        <<<(unsigned)((n + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    using T = decltype(t);
+    using C = decltype(e);
+    if (rows) {
+      const int h = halves ? (int)half : 0;
+      const RowJobs turned{Divider((D - h) / 8), h}, plain{Divider(D / 8), 0};
+      const int rope4 = rotates && a->rope_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a->cos) % 16 == 0 &&
+                        reinterpret_cast<uintptr_t>(a->sin) % 16 == 0;
+      // one warp a token when that fills the SMs (16 warps each), else up to 8 warps
+      p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(8, 148 * 16 / a->tokens));
+      append_rows_kernel<T, C><<<dim3((unsigned)((a->tokens + 3) / 4), p.parts), 128, 0, st>>>(p, turned, plain, rope4);
+    } else if (columns && a->tokens <= 65535 * 32) {
+      // at most 32 tokens a block, fewer for more blocks, but whole 32-byte sectors of a feature's tokens
+      const int fewest = sizeof(T) == 4 ? 3 : 4;
+      p.tile_bits = 5;
+      while (p.tile_bits > fewest && heads * (a->tokens >> p.tile_bits) < 4 * 148) --p.tile_bits;
+      while (p.tile_bits > 2 && a->tokens <= 1 << (p.tile_bits - 1)) --p.tile_bits;
+      const Divider pairs(D / 2);
+      p.pairs_mul = pairs.mul, p.pairs_shift = pairs.shift;
+      append_columns_kernel<T, C>
+          <<<dim3((unsigned)heads, (unsigned)((a->tokens + (1 << p.tile_bits) - 1) >> p.tile_bits)), 256, 0, st>>>(p);
+    } else {
+      append_any_kernel<T, C><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p);
+    }
   });
   cuda_check(cudaGetLastError(), "launch cache append");
   SC_SERVE_END

@@ -48,7 +48,8 @@ def _rows(t, name: str, device: int, shape, dtype) -> tuple:
 
 
 def _apart(t, name: str) -> None:
-    if 0 in t.stride() and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+    strides = t.stride()
+    if 0 in strides and any(st == 0 and n > 1 for st, n in zip(strides, t.shape)):
         _fail(f"{name} has elements that share memory")
 
 
@@ -70,20 +71,24 @@ def _table(t, device: int) -> tuple:
 
 
 def _on(stream, device: int, *tensors) -> int:
-    """The raw stream of a call; tensors that are used on another stream than
-    torch's current one are kept from reuse until that stream is done with them."""
-    current = torch.cuda.current_stream(device)
-    if stream is None or stream.cuda_stream == current.cuda_stream:
-        return current.cuda_stream
-    for t in tensors:
-        if t is not None:
-            t.record_stream(stream)
+    """The raw stream of a call on ``stream``; the tensors that it uses there are
+    kept from reuse until that stream is done with them."""
+    if stream.cuda_stream != _current(device):
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
     return stream.cuda_stream
+
+
+# torch.cuda.current_stream builds an object (1.2 us a call); the raw handle is all that a launch needs.
+_current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 class _Handle:
     _free = ""
     _status = ""
+    _run = ""
     _h: Optional[ctypes.c_void_p] = None
 
     def status(self) -> int:
@@ -104,6 +109,7 @@ class _Handle:
     def _own(self, h: ctypes.c_void_p) -> None:
         self._h = h
         self._release = getattr(lib(), self._free)  # module globals may be gone when the interpreter ends
+        self._call = getattr(lib(), self._run)
 
     def __del__(self):
         if self._h is not None:
@@ -136,7 +142,7 @@ class PagedKVCache(_Handle):
     16-byte boundary; a permuted [num_pages, page_size, kv_heads, head_dim]
     pool is taken too.  Row i of a page table lists the pages of sequence i.
     """
-    _free, _status = "sc_kv_cache_free", "sc_kv_cache_status"
+    _free, _status, _run = "sc_kv_cache_free", "sc_kv_cache_status", "sc_kv_append"
 
     def __init__(self, k, v):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
@@ -191,7 +197,7 @@ class PagedKVCache(_Handle):
             qshape = (n, heads, self.head_dim)
             qa = _rows(q, "q", dev, qshape, dtype)
             if q_out is None:
-                q_out = torch.empty(qshape, dtype=dtype, device=q.device)
+                q_out = q.new_empty(qshape)
             oa = _rows(q_out, "q_out", dev, qshape, dtype)
             _apart(q_out, "q_out")
             if n and oa[0] == qa[0] and oa != qa:
@@ -207,10 +213,12 @@ class PagedKVCache(_Handle):
             if n:
                 _fail("an empty page table")
             return q_out
-        s = _on(stream, dev, k, v, positions, seq_ids, page_table, q, q_out, self.k, self.v,
-                *((rope.cos, rope.sin) if rope is not None else ()))
-        _check(lib().sc_kv_append(self._h, _APPEND.pack(n, heads, kind, *ka, *va, *qa, *oa, pos, ids, tab, seqs, cols,
-                                                        tstride, *ra), s))
+        s = _current(dev) if stream is None else _on(stream, dev, k, v, positions, seq_ids, page_table, q, q_out, self.k,
+                                                     self.v, *((rope.cos, rope.sin) if rope is not None else ()))
+        bad = self._call(self._h, _APPEND.pack(n, heads, kind, *ka, *va, *qa, *oa, pos, ids, tab, seqs, cols, tstride,
+                                               *ra), s)
+        if bad:
+            _check(bad)
         return q_out
 
 
@@ -221,7 +229,7 @@ class DecodeAttention(_Handle):
     ``scale`` defaults to 1/sqrt(head_dim); ``window`` > 0 limits a sequence
     to its last ``window`` keys.  Calls share the plan's workspace: use one
     plan per stream."""
-    _free, _status = "sc_attn_free", "sc_attn_status"
+    _free, _status, _run = "sc_attn_free", "sc_attn_status", "sc_attn_decode"
 
     def __init__(self, cache: PagedKVCache, q_heads: int, max_seqs: int, scale: Optional[float] = None,
                  window: int = 0):
@@ -248,18 +256,21 @@ class DecodeAttention(_Handle):
         shape = (n, self.q_heads, self.cache.head_dim)
         qa = _rows(q, "q", dev, shape, dtype)
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=q.device)
+            out = q.new_empty(shape)
         oa = _rows(out, "out", dev, shape, dtype)
         _apart(out, "out")
         tab, rows, cols, tstride = _table(page_table, dev)
         if rows < n:
             _fail(f"{n} sequences need a page table of as many rows, got {rows}")
         lens = _ints(seq_lens, "seq_lens", dev, n)
-        lse = torch.empty((n, self.q_heads), dtype=torch.float32, device=q.device) if return_lse else None
+        lse = q.new_empty((n, self.q_heads), dtype=torch.float32) if return_lse else None
         if n:
-            s = _on(stream, dev, q, out, page_table, seq_lens, lse, self.cache.k, self.cache.v)
-            _check(lib().sc_attn_decode(self._h, _ATTEND.pack(n, kind, *qa, *oa, lse.data_ptr() if return_lse else 0,
-                                                              tab, cols, tstride, lens), s))
+            s = _current(dev) if stream is None else _on(stream, dev, q, out, page_table, seq_lens, lse, self.cache.k,
+                                                         self.cache.v)
+            bad = self._call(self._h, _ATTEND.pack(n, kind, *qa, *oa, lse.data_ptr() if return_lse else 0, tab, cols,
+                                                   tstride, lens), s)
+            if bad:
+                _check(bad)
         return (out, lse) if return_lse else out
 
 
@@ -269,7 +280,7 @@ class LowRankAdapters(_Handle):
     down[i] [rank_i, in_features] and up[i] [out_features, rank_i] of one type
     (fp32, fp16, bf16) and ranks of 0 to 256.  The weights are copied into the
     set's own layout once."""
-    _free, _status = "sc_adapters_free", "sc_adapters_status"
+    _free, _status, _run = "sc_adapters_free", "sc_adapters_status", "sc_adapters_apply"
 
     def __init__(self, down: Sequence, up: Sequence, scales: Sequence[float]):
         n = len(down)
@@ -326,8 +337,7 @@ class LowRankAdapters(_Handle):
         ba = (0, 0, 0) if base is None else _rows(base, "base", dev, shape, dtype)
         if out is None:
             # laid out as x is: feature-major, or token-major from a transposed x
-            out = torch.empty((n, self.out_features), dtype=dtype, device=x.device).t() \
-                if xa[1] == 1 and n > 1 else torch.empty(shape, dtype=dtype, device=x.device)
+            out = x.new_empty((n, self.out_features)).t() if xa[1] == 1 and n > 1 else x.new_empty(shape)
         oa = _rows(out, "out", dev, shape, dtype)
         _apart(out, "out")
         if n and oa[0] == ba[0] and oa != ba:
@@ -337,8 +347,9 @@ class LowRankAdapters(_Handle):
         idp = _ints(ids, "ids", dev, n)
         if n:
             size = self._workspace(n)
-            work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-            s = _on(stream, dev, x, ids, base, out, work)
-            _check(lib().sc_adapters_apply(self._h, _ADAPT.pack(n, kind, *xa, *ba, *oa, idp,
-                                                                work.data_ptr() if size else 0, size), s))
+            work = x.new_empty(size, dtype=torch.uint8) if size else None
+            s = _current(dev) if stream is None else _on(stream, dev, x, ids, base, out, work)
+            bad = self._call(self._h, _ADAPT.pack(n, kind, *xa, *ba, *oa, idp, work.data_ptr() if size else 0, size), s)
+            if bad:
+                _check(bad)
         return out
