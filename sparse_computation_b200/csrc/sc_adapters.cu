@@ -1,15 +1,19 @@
 // Low-rank adapters of many requests beside a shared projection.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <memory>
+#include <type_traits>
 #include <vector>
 
 #include <cooperative_groups.h>
 
+#include "sc_mma.cuh"
 #include "sc_serve.h"
 
 using namespace sc::serve;
 namespace cg = cooperative_groups;
+namespace mma = sc::mma;
 
 namespace {
 
@@ -38,80 +42,44 @@ __global__ void pack_rows(const W *src, int64_t row_stride, int64_t col_stride, 
   if (r < rows) dst[i] = c < cols ? src[r * row_stride + c * col_stride] : W(0);
 }
 
-__device__ __forceinline__ int adapter_of(const SetView &s, const int32_t *ids, int64_t t) {
-  const int a = ids[t];
-  if (a >= s.count) {
-    set_status(s.status, 10);
-    return -1;
-  }
-  return a;
-}
-
-// One warp per (token, rank row): v = scale * down x.
-template <class T, class W>
-__global__ void __launch_bounds__(256) shrink_kernel(const SetView s, const sc_adapters_args a, float *v) {
-  const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32;
-  const int lane = threadIdx.x % 32;
-  if (i >= a.tokens * s.rank_max) return;
-  const int64_t t = i / s.rank_max, r = i % s.rank_max;
-  const int ad = adapter_of(s, a.ids, t);
-  if (ad < 0 || r >= s.first[ad + 1] - s.first[ad]) return;
-  const W *w = static_cast<const W *>(s.down) + (s.first[ad] + r) * s.in_row;
-  const T *x = static_cast<const T *>(a.x.ptr) + t * a.x.stride[1];
-  float sum = 0.f;
-  for (int64_t k = lane; k < s.in; k += 32) sum += to_f32(w[k]) * to_f32(x[k * a.x.stride[0]]);
-  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-  if (lane == 0) v[i] = sum * s.scale[ad];
-}
-
-// One thread per output element: out = base + up v.
-template <class T, class W>
-__global__ void __launch_bounds__(256) expand_kernel(const SetView s, const sc_adapters_args a, const float *v) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= a.tokens * s.out) return;
-  const int64_t t = i / s.out, m = i % s.out;
-  float y = 0.f;
-  if (a.base.ptr) y = to_f32(static_cast<const T *>(a.base.ptr)[m * a.base.stride[0] + t * a.base.stride[1]]);
-  const int ad = adapter_of(s, a.ids, t);
-  if (ad >= 0) {
-    const int r0 = s.first[ad], n = s.first[ad + 1] - r0;
-    float sum = 0.f;
-    for (int r = 0; r < n; ++r)
-      sum += v[t * s.rank_max + r] * to_f32(static_cast<const W *>(s.up)[(int64_t)(r0 + r) * s.out_row + m]);
-    y += sum;
-  }
-  static_cast<T *>(a.out.ptr)[m * a.out.stride[0] + t * a.out.stride[1]] = from_f32<T>(y);
-}
-
 // ------------------------------------------------------ a few tokens ----
 //
 // Up to kFewTokens tokens (a decoding step): what counts is reading each
-// adapter's weights once and at once.  A cluster of eight blocks takes up to
-// eight tokens that share an adapter: the cluster of a token whose place among
-// its adapter's tokens is a multiple of eight takes that one and the next
-// seven, the others' clusters leave.  Block c multiplies columns c of eight
-// parts of `down` with its part of x, so that x is read once, too; the eight
-// parts of v = down x are added up through distributed shared memory, in block
-// order; then block c makes rows c of eight parts of up v.  One launch, no
-// scratch memory.  Bound by the weights' bytes, and by latency below some MB.
-constexpr int kFewTokens = 256, kCluster = 8, kGroup = 8, kChunk = 512, kFewThreads = 256;
+// adapter's weights once and at once.  A cluster of two to eight blocks takes
+// up to kGroup tokens that share an adapter: the cluster of a token whose
+// place among its adapter's tokens is a multiple of kGroup takes that one and
+// the next ones, the others leave.  Each block multiplies its part of the
+// columns of `down` with its part of x, so that x is read once; the parts of
+// v = down x are added up through distributed shared memory, in block order;
+// then each block makes its part of the rows of up v.  One launch, no scratch
+// memory.  Bound by latency (a chain of ids, weights, two cluster barriers,
+// weights) and fp32 instructions; the tensor-core tiles below have twice the
+// fixed cost: 128 tokens of 100 adapters of 512 x 2048 take 14.3 us here, 28.6
+// there.
+constexpr int kFewTokens = 256, kGroup = 4, kFewChunk = 512, kFewThreads = 256, kFewBlocks = 3;
 
-// Eight weights as floats.
+// Eight weights, as they lie.
 template <class W>
-__device__ __forceinline__ void load8(const W *p, float (&x)[8]) {
+struct Eight {
   uint4 w[sizeof(W) / 2];
+  __device__ __forceinline__ void load(const W *p) {
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(W) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
-  const W *v = reinterpret_cast<const W *>(w);
+    for (int i = 0; i < (int)sizeof(W) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const W *v = reinterpret_cast<const W *>(w);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_f32(v[i]);
-}
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(v[i]);
+  }
+};
 
 struct FewShared {
-  float x[kGroup][kChunk];          // this block's part of the tokens' x
-  float part[kMaxRank][kGroup];     // its part of v, read by the whole cluster
-  float v[kMaxRank][kGroup];        // scale * v
-  float sums[kFewThreads * 8];
+  union {
+    float x[kGroup][kFewChunk];           // this block's part of the tokens' x
+    float sums[kGroup][kFewThreads * 8];  // parts of up v
+  };
+  float part[kMaxRank][kGroup];  // its part of v, read by the whole cluster
+  float v[kMaxRank][kGroup];     // scale * v
   int tokens[kGroup];
   int count[kFewThreads / 32], n;
 };
@@ -124,24 +92,41 @@ __device__ __forceinline__ void few_shrink(FewShared &sh, const W *down, int64_t
   int lanes = 32;
   while (lanes > 1 && lanes * 4 >= width) lanes >>= 1;
   const int sub = lane / lanes, in = lane % lanes, rows = 32 / lanes;
-  for (int r0 = warp * rows; r0 < rank; r0 += kFewThreads / 32 * rows) {
-    const int r = r0 + sub;
-    float acc[NT] = {};
-    if (r < rank)
-      for (int k = in * 8; k < width; k += lanes * 8) {
-        float w[8];
-        load8(down + r * row + k, w);
+  constexpr int B = 4, warps = kFewThreads / 32;  // B rows of a lane at a time
+  for (int r0 = warp * rows; r0 < rank; r0 += B * warps * rows) {
+    float acc[B][NT] = {};
+    for (int k = in * 8; k < width; k += lanes * 8) {
+      Eight<W> w[B];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float4 a = *reinterpret_cast<const float4 *>(&sh.x[t][k]);
-          const float4 b = *reinterpret_cast<const float4 *>(&sh.x[t][k + 4]);
-          acc[t] += w[0] * a.x + w[1] * a.y + w[2] * a.z + w[3] * a.w + w[4] * b.x + w[5] * b.y + w[6] * b.z + w[7] * b.w;
-        }
+      for (int i = 0; i < B; ++i) {
+        const int r = r0 + i * warps * rows + sub;
+        w[i].load(down + min(r, rank - 1) * row + k);
       }
+      float x[NT][8];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      for (int d = lanes / 2; d; d >>= 1) acc[t] += __shfl_xor_sync(~0u, acc[t], d);
-      if (in == 0 && r < rank) sh.part[r][t] += acc[t];
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) *reinterpret_cast<float4 *>(&x[t][e]) = *reinterpret_cast<const float4 *>(&sh.x[t][k + e]);
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        if (r0 + i * warps * rows >= rank) break;
+        float f[8];
+        w[i].get(f);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[i][t] += f[e] * x[t][e];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const int r = r0 + i * warps * rows + sub;
+      if (r - sub >= rank) break;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        for (int d = lanes / 2; d; d >>= 1) acc[i][t] += __shfl_xor_sync(~0u, acc[i][t], d);
+        if (in == 0 && r < rank) sh.part[r][t] += acc[i][t];
+      }
     }
   }
 }
@@ -151,56 +136,80 @@ __device__ __forceinline__ void few_shrink(FewShared &sh, const W *down, int64_t
 template <int NT, class T, class W>
 __device__ __forceinline__ void few_expand(FewShared &sh, const sc_adapters_args &a, const W *up, int64_t row, int rank, int m0,
                                            int rows) {
+  constexpr int kEarly = 2;  // values of base that a thread asks for ahead
+  float early[NT][kEarly] = {};
+  if (a.base.ptr)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < kEarly; ++j) {
+        const int i = threadIdx.x + j * kFewThreads;
+        if (t < sh.n && i < rows)
+          early[t][j] = to_f32(static_cast<const T *>(a.base.ptr)[(int64_t)(m0 + i) * a.base.stride[0] +
+                                                                  (int64_t)sh.tokens[t] * a.base.stride[1]]);
+      }
   for (int base = 0; base < rows; base += kFewThreads * 8) {
     const int here = min(rows - base, kFewThreads * 8), eights = (here + 7) / 8;
     const int sets = kFewThreads / eights, set = threadIdx.x / eights, at = base + threadIdx.x % eights * 8;
     float acc[NT][8] = {};
+    constexpr int B = NT <= 2 && sizeof(W) == 2 ? 8 : 4;  // rank rows of a thread at a time
     if (set < sets)
-#pragma unroll 4
-      for (int r = set; r < rank; r += sets) {
-        float w[8];
-        load8(up + r * row + m0 + at, w);
+      for (int r0 = set; r0 < rank; r0 += B * sets) {
+        Eight<W> w[B];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float v = sh.v[r][t];
+        for (int i = 0; i < B; ++i) w[i].load(up + min(r0 + i * sets, rank - 1) * row + m0 + at);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) acc[t][e] += w[e] * v;
+        for (int i = 0; i < B; ++i) {
+          if (r0 + i * sets >= rank) break;
+          float f[8];
+          w[i].get(f);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const float v = sh.v[r0 + i * sets][t];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[t][e] += f[e] * v;
+          }
         }
       }
+    __syncthreads();
+    if (set < sets)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (t >= sh.n) break;
-      __syncthreads();
-      if (set < sets)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 8; e += 4)
-          *reinterpret_cast<float4 *>(&sh.sums[set * eights * 8 + at - base + e]) =
+          *reinterpret_cast<float4 *>(&sh.sums[t][set * eights * 8 + at - base + e]) =
               make_float4(acc[t][e], acc[t][e + 1], acc[t][e + 2], acc[t][e + 3]);
-      __syncthreads();
-      const int64_t token = sh.tokens[t];
-      for (int i = threadIdx.x; i < here; i += kFewThreads) {
-        const int64_t m = m0 + base + i;
+    __syncthreads();
+    for (int i = threadIdx.x, j = 0; i < here; i += kFewThreads, ++j) {
+      const int64_t m = m0 + base + i;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (t >= sh.n) break;
+        const int64_t token = sh.tokens[t];
         float y = 0.f;
-        for (int s = 0; s < sets; ++s) y += sh.sums[s * eights * 8 + i];
-        if (a.base.ptr) y += to_f32(static_cast<const T *>(a.base.ptr)[m * a.base.stride[0] + token * a.base.stride[1]]);
+        for (int s = 0; s < sets; ++s) y += sh.sums[t][s * eights * 8 + i];
+        if (a.base.ptr)
+          y += j < kEarly && base == 0
+                   ? early[t][j < kEarly ? j : 0]
+                   : to_f32(static_cast<const T *>(a.base.ptr)[m * a.base.stride[0] + token * a.base.stride[1]]);
         static_cast<T *>(a.out.ptr)[m * a.out.stride[0] + token * a.out.stride[1]] = from_f32<T>(y);
       }
     }
+    __syncthreads();
   }
 }
 
 template <class T, class W>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFewThreads)
-    few_kernel(const __grid_constant__ SetView s, const __grid_constant__ sc_adapters_args a) {
+__global__ void __launch_bounds__(kFewThreads, kFewBlocks) few_kernel(const __grid_constant__ SetView s, const __grid_constant__ sc_adapters_args a) {
   __shared__ FewShared sh;
-  const int c = blockIdx.x, t = blockIdx.y, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int c = blockIdx.x, blocks = gridDim.x, t = blockIdx.y, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int n_tokens = (int)a.tokens;
   const int id = a.ids[t];
   const int other = tid < n_tokens ? a.ids[tid] : -1;
   const int rank = id >= 0 && id < s.count ? s.first[id + 1] - s.first[id] : 0;
   // this block's columns of x and rows of out
-  const int k0 = (int)(s.in_row / kCluster) * c, k1 = min((int)s.in, k0 + (int)(s.in_row / kCluster));
-  const int m0 = (int)(s.out_row / kCluster) * c, m1 = min((int)s.out, m0 + (int)(s.out_row / kCluster));
+  const int k0 = (int)(s.in_row / blocks) * c, k1 = min((int)s.in, k0 + (int)(s.in_row / blocks));
+  const int m0 = (int)(s.out_row / blocks) * c, m1 = min((int)s.out, m0 + (int)(s.out_row / blocks));
   if (rank == 0) {
     if (id >= s.count && c == 0 && tid == 0) set_status(s.status, 10);
     if (a.out.ptr != a.base.ptr)
@@ -229,24 +238,40 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFewThreads)
   for (int i = tid; i < rank * kGroup; i += kFewThreads) sh.part[i / kGroup][i % kGroup] = 0.f;
   __syncthreads();
   const int n = sh.n;
-  const W *down = static_cast<const W *>(s.down) + s.first[id] * s.in_row, *up = static_cast<const W *>(s.up) + s.first[id] * s.out_row;
-  for (int k = k0; k < k1; k += kChunk) {
-    const int width = min(kChunk, k1 - k), wide = (width + 7) / 8 * 8;
-    for (int i = tid; i < kGroup * wide; i += kFewThreads) {
-      const int g = i / wide, kk = i - g * wide;
-      sh.x[g][kk] = g < n && kk < width
-                        ? to_f32(static_cast<const T *>(a.x.ptr)[(k + kk) * a.x.stride[0] + sh.tokens[g] * a.x.stride[1]])
-                        : 0.f;
-    }
+  const W *down = static_cast<const W *>(s.down) + s.first[id] * s.in_row,
+          *up = static_cast<const W *>(s.up) + s.first[id] * s.out_row;
+  // the second product's weights on their way to L2 while the first one runs
+  if (m1 > m0) {
+    const int lines = (int)((m1 - m0) * sizeof(W) + 127) / 128;
+    for (int i = tid; i < rank * lines; i += kFewThreads)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint8_t *>(up + (int64_t)(i / lines) * s.out_row + m0) +
+                                                   i % lines * 128));
+  }
+  for (int k = k0; k < k1; k += kFewChunk) {
+    const int width = min(kFewChunk, k1 - k), wide = (width + 7) / 8 * 8;
+    constexpr int per = kFewChunk / kFewThreads;
+    float x[kGroup][per];  // all loads at once
+#pragma unroll
+    for (int g = 0; g < kGroup; ++g)
+#pragma unroll
+      for (int i = 0; i < per; ++i) {
+        const int kk = tid + i * kFewThreads;
+        x[g][i] = g < n && kk < width
+                      ? to_f32(static_cast<const T *>(a.x.ptr)[(k + kk) * a.x.stride[0] + sh.tokens[g] * a.x.stride[1]])
+                      : 0.f;
+      }
+#pragma unroll
+    for (int g = 0; g < kGroup; ++g)
+#pragma unroll
+      for (int i = 0; i < per; ++i)
+        if (tid + i * kFewThreads < wide) sh.x[g][tid + i * kFewThreads] = x[g][i];
     __syncthreads();
     if (n == 1)
       few_shrink<1>(sh, down + k, s.in_row, rank, wide);
     else if (n == 2)
       few_shrink<2>(sh, down + k, s.in_row, rank, wide);
-    else if (n <= 4)
-      few_shrink<4>(sh, down + k, s.in_row, rank, wide);
     else
-      few_shrink<8>(sh, down + k, s.in_row, rank, wide);
+      few_shrink<kGroup>(sh, down + k, s.in_row, rank, wide);
     __syncthreads();
   }
   cg::cluster_group cluster = cg::this_cluster();
@@ -254,7 +279,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFewThreads)
   const float scale = s.scale[id];
   for (int i = tid; i < rank * kGroup; i += kFewThreads) {
     float v = 0.f;
-    for (int b = 0; b < kCluster; ++b) v += cluster.map_shared_rank(&sh.part[0][0], b)[i];
+    for (int b = 0; b < blocks; ++b) v += cluster.map_shared_rank(&sh.part[0][0], b)[i];
     sh.v[i / kGroup][i % kGroup] = v * scale;
   }
   cluster.sync();  // no block leaves, or goes on, before all have read
@@ -263,10 +288,403 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFewThreads)
     few_expand<1, T>(sh, a, up, s.out_row, rank, m0, m1 - m0);
   else if (n == 2)
     few_expand<2, T>(sh, a, up, s.out_row, rank, m0, m1 - m0);
-  else if (n <= 4)
-    few_expand<4, T>(sh, a, up, s.out_row, rank, m0, m1 - m0);
   else
-    few_expand<8, T>(sh, a, up, s.out_row, rank, m0, m1 - m0);
+    few_expand<kGroup, T>(sh, a, up, s.out_row, rank, m0, m1 - m0);
+}
+
+// ---------------------------------------------------- prompts ----
+//
+// A cluster of two to eight blocks takes a tile: up to kTile tokens that share
+// an adapter.  Each block multiplies its part of the columns of `down` with its
+// part of x, so that x is read once; the parts of v = down x are added up
+// through distributed shared memory, in block order; then each block makes its
+// part of the rows of up v.  One launch; v never leaves the chip.
+//
+// Both products are mma.sync with the tokens as the 16 rows and the weights
+// straight from global memory into B fragments, as whole 16-byte pieces per
+// lane (the sum over columns may run in any order, and so may the rows of the
+// result): of `down`, piece t + 4j of rank row g; of `up` (stored transposed),
+// the piece at rows 8g.. of ranks 2t, 2t+1 (+8).  What a 16-bit operand loses
+// of x and v goes into further parts, one instruction each (two TF32 parts on
+// both sides for fp32 weights), fp16 parts scaled by a power of two.  The same
+// with fp32 instructions took 22.5 us for 96 tokens of 40 adapters of
+// 4096 x 4096, bound by instructions; this takes TODO.
+//
+// A block sorts the tokens by adapter first (group_kernel); tokens without one
+// are copied.  Bound by x and out at best, at present by instructions and the
+// barriers between the phases of a tile.
+constexpr int kMaxCluster = 8, kTile = 16, kChunk = 512, kThreads = 256, kWarps = kThreads / 32;
+constexpr int kXRow = kChunk + 4, kSpan = 64;  // floats of a token's chunk in shared memory; columns of a warp
+
+struct Tile {
+  int adapter, first, n;  // first: in the sorted tokens
+};
+
+// The tokens sorted by adapter, and the tiles that they are cut into.
+struct Sorted {
+  const Tile *tiles;  // *n of them
+  const int *tokens, *n;
+};
+
+template <class T, class W>
+struct Kind {
+  static constexpr bool f32 = sizeof(W) == 4, f16 = std::is_same<W, __half>::value, same = std::is_same<T, W>::value && !f32;
+  static constexpr int mode = f32 ? mma::kTF32 : f16 ? mma::kF16Wide : mma::kBF16Wide;
+  static constexpr int px = same ? 1 : f32 || f16 ? 2 : 3;                      // parts of x
+  static constexpr int pv = f32 || f16 ? 2 : sizeof(T) == 2 ? 2 : 3;            // of v
+  static constexpr int epc = 16 / sizeof(W), J = kSpan / (4 * epc);             // elements of a piece, pieces of a lane
+  static constexpr int unit = 8 * epc;                                          // rows of `up` that a warp makes at a time
+  static constexpr int step = f32 ? 8 : 16;                                     // ranks of an instruction
+  static constexpr bool scaled = f16 && !same;
+};
+
+// The power of two that brings top to below 2.
+__device__ __forceinline__ float scale_to_two(float top) {
+  const int e = (int)(__float_as_uint(top) >> 23) - 127;
+  return e > -120 && e < 127 ? __uint_as_float((uint32_t)(e + 127) << 23) : 1.f;
+}
+
+// Two neighbouring values of rows g and g + 8 as parts of A: a[part][0] row g, [1] row g + 8.
+template <int MODE, int PARTS>
+__device__ __forceinline__ void split2(float x0, float x1, float y0, float y1, uint32_t (&a)[PARTS][2]) {
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    a[p][0] = mma::pack2<MODE>(x0, x1);
+    a[p][1] = mma::pack2<MODE>(y0, y1);
+  }
+}
+
+template <class T, class W>
+__global__ void __launch_bounds__(kThreads, 2)
+    tile_kernel(const __grid_constant__ SetView s, const __grid_constant__ sc_adapters_args a, const Sorted sorted) {
+  using K = Kind<T, W>;
+  extern __shared__ __align__(16) float smem[];
+  __shared__ int s_tokens[kTile];
+  const int c = blockIdx.x, blocks = gridDim.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
+  // this block's columns of x and rows of out
+  const int k0 = (int)(s.in_row / blocks) * c, k1 = min((int)s.in, k0 + (int)(s.in_row / blocks));
+  const int m0 = (int)(s.out_row / blocks) * c, m1 = min((int)s.out, m0 + (int)(s.out_row / blocks));
+  if ((int)blockIdx.y >= *sorted.n) return;  // the whole cluster
+  const Tile tile = sorted.tiles[blockIdx.y];
+  const int id = tile.adapter, n = tile.n;
+  if (tid < n) s_tokens[tid] = sorted.tokens[tile.first + tid];
+  __syncthreads();
+  if (id < 0) {
+    if (a.out.ptr == a.base.ptr) return;
+    const bool by_token = a.out.stride[1] == 1;
+    const int rows = m1 - m0;
+    for (int i = tid; i < rows * n; i += kThreads) {
+      const int64_t m = m0 + (by_token ? i / n : i % rows), tok = s_tokens[by_token ? i % n : i / rows];
+      static_cast<T *>(a.out.ptr)[m * a.out.stride[0] + tok * a.out.stride[1]] =
+          a.base.ptr ? static_cast<const T *>(a.base.ptr)[m * a.base.stride[0] + tok * a.base.stride[1]] : from_f32<T>(0.f);
+    }
+    return;
+  }
+  const int first = s.first[id], rank = s.first[id + 1] - first;
+  const float scale = s.scale[id];
+  const W *down = static_cast<const W *>(s.down) + first * s.in_row, *up = static_cast<const W *>(s.up) + first * s.out_row;
+  // the second product's weights on their way to L2 while the first one runs
+  if (m1 > m0) {
+    const int lines = (int)((m1 - m0) * sizeof(W) + 127) / 128;
+    for (int i = tid; i < rank * lines; i += kThreads)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint8_t *>(up + (int64_t)(i / lines) * s.out_row + m0) +
+                                                   i % lines * 128));
+  }
+  const int v_row = (rank + 15) / 16 * 16 + 4;  // floats; ranks up to a multiple of 16 are zeros
+  float *x_tile = smem, *part = smem + kTile * kXRow, *v_part = part + kWarps * kTile * 64;
+  float *v = part;  // after the parts are added up
+  for (int i = tid; i < kTile * v_row; i += kThreads) v_part[i] = 0.f;
+
+  // ---- v = down x over this block's columns, kChunk at a time
+  for (int k = k0; k < k1; k += kChunk) {
+    const int width = min(kChunk, k1 - k);
+    const bool by_token = a.x.stride[1] == 1;  // neighbouring threads on neighbouring tokens, else on neighbouring features
+    __syncthreads();
+#pragma unroll 1
+    for (int i0 = tid; i0 < kTile * kChunk; i0 += 8 * kThreads) {
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * kThreads, row = by_token ? i % kTile : i / kChunk, col = by_token ? i / kTile : i % kChunk;
+        x[u] = row < n && col < width
+                   ? to_f32(static_cast<const T *>(a.x.ptr)[(k + col) * a.x.stride[0] + (int64_t)s_tokens[row] * a.x.stride[1]])
+                   : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * kThreads, row = by_token ? i % kTile : i / kChunk, col = by_token ? i / kTile : i % kChunk;
+        if (col < (width + kSpan - 1) / kSpan * kSpan) x_tile[row * kXRow + col] = x[u];
+      }
+      if ((by_token ? (i0 - tid + 8 * kThreads) / kTile : 0) >= (width + kSpan - 1) / kSpan * kSpan) break;
+    }
+    __syncthreads();
+    // warps: kw of them along the columns, kSpan each, the others along the ranks
+    const int spans = (width + kSpan - 1) / kSpan, kw = spans > 4 ? 8 : spans > 2 ? 4 : spans;
+    const int col0 = warp % kw * kSpan;
+    const bool busy = col0 < spans * kSpan;
+    uint32_t ax[K::J][2][K::px][4];  // A fragments: of pieces, their two k-steps
+    float up_g = 1.f, up_g8 = 1.f;
+    if (busy) {
+      float xs[K::J][2][K::epc];
+#pragma unroll
+      for (int j = 0; j < K::J; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < K::epc; e += 4) {
+            const float4 y = *reinterpret_cast<const float4 *>(&x_tile[(g + 8 * h) * kXRow + col0 + (t + 4 * j) * K::epc + e]);
+            xs[j][h][e] = y.x, xs[j][h][e + 1] = y.y, xs[j][h][e + 2] = y.z, xs[j][h][e + 3] = y.w;
+          }
+      if (K::scaled) {
+        float top[2] = {0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int j = 0; j < K::J; ++j)
+#pragma unroll
+            for (int e = 0; e < K::epc; ++e) top[h] = fmaxf(top[h], fabsf(xs[j][h][e]));
+          top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
+          top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
+        }
+        up_g = scale_to_two(top[0]);
+        up_g8 = scale_to_two(top[1]);
+#pragma unroll
+        for (int j = 0; j < K::J; ++j)
+#pragma unroll
+          for (int e = 0; e < K::epc; ++e) xs[j][0][e] *= 1.f / up_g, xs[j][1][e] *= 1.f / up_g8;
+      }
+#pragma unroll
+      for (int j = 0; j < K::J; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (K::f32) {
+            const float x0 = xs[j][0][2 * h], x1 = xs[j][0][2 * h + 1], y0 = xs[j][1][2 * h], y1 = xs[j][1][2 * h + 1];
+            ax[j][h][0][0] = mma::tf32_head(x0), ax[j][h][0][1] = mma::tf32_head(y0);
+            ax[j][h][0][2] = mma::tf32_head(x1), ax[j][h][0][3] = mma::tf32_head(y1);
+            ax[j][h][K::px - 1][0] = mma::tf32_tail(x0), ax[j][h][K::px - 1][1] = mma::tf32_tail(y0);
+            ax[j][h][K::px - 1][2] = mma::tf32_tail(x1), ax[j][h][K::px - 1][3] = mma::tf32_tail(y1);
+          } else {
+            constexpr int q = K::epc / 2;
+            uint32_t lo[K::px][2], hi[K::px][2];
+            split2<K::mode>(xs[j][0][q * h], xs[j][0][q * h + 1], xs[j][1][q * h], xs[j][1][q * h + 1], lo);
+            split2<K::mode>(xs[j][0][q * h + q - 2], xs[j][0][q * h + q - 1], xs[j][1][q * h + q - 2], xs[j][1][q * h + q - 1], hi);
+#pragma unroll
+            for (int p = 0; p < K::px; ++p) {
+              ax[j][h][p][0] = lo[p][0], ax[j][h][p][1] = lo[p][1];
+              ax[j][h][p][2] = hi[p][0], ax[j][h][p][3] = hi[p][1];
+            }
+          }
+        }
+    }
+    const int row_end = (int)s.in_row - k;  // columns from k on that a weight row has
+    for (int r64 = 0; r64 < rank; r64 += 64) {
+      const int tiles = (min(64, rank - r64) + 7) / 8, across = kWarps / kw, mine = warp / kw;
+      if (busy) {
+        constexpr int B = 4;  // rank tiles whose weights are in flight
+#pragma unroll 1
+        for (int nt0 = mine; nt0 < tiles; nt0 += B * across) {
+          uint4 w[B][K::J];
+#pragma unroll
+          for (int i = 0; i < B; ++i) {
+            const W *row = down + (int64_t)min(r64 + (nt0 + i * across) * 8 + g, rank - 1) * s.in_row + k;
+#pragma unroll
+            for (int j = 0; j < K::J; ++j) {
+              const int col = col0 + (t + 4 * j) * K::epc;
+              w[i][j] = __ldg(reinterpret_cast<const uint4 *>(row + (col < row_end ? col : 0)));  // beyond: x is zero
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < B; ++i) {
+            if (nt0 + i * across >= tiles) break;
+            float acc[2][4] = {};
+#pragma unroll
+            for (int j = 0; j < K::J; ++j) {
+              const uint32_t b[4] = {w[i][j].x, w[i][j].y, w[i][j].z, w[i][j].w};
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int p = 0; p < K::px; ++p) {
+                  const uint32_t(&f)[4] = ax[j][h][p];
+                  if (K::f32) {
+                    const float b0 = __uint_as_float(b[2 * h]), b1 = __uint_as_float(b[2 * h + 1]);
+                    mma::mma16<K::mode>(acc[0], f[0], f[1], f[2], f[3], mma::tf32_head(b0), mma::tf32_head(b1));
+                    if (p == 0) mma::mma16<K::mode>(acc[1], f[0], f[1], f[2], f[3], mma::tf32_tail(b0), mma::tf32_tail(b1));
+                  } else {
+                    mma::mma16<K::mode>(acc[h], f[0], f[1], f[2], f[3], b[2 * h], b[2 * h + 1]);
+                  }
+                }
+            }
+            float *to = part + ((warp % kw) * kTile + g) * 64 + (nt0 + i * across) * 8 + 2 * t;
+            *reinterpret_cast<float2 *>(to) = make_float2((acc[0][0] + acc[1][0]) * up_g, (acc[0][1] + acc[1][1]) * up_g);
+            *reinterpret_cast<float2 *>(to + 8 * 64) =
+                make_float2((acc[0][2] + acc[1][2]) * up_g8, (acc[0][3] + acc[1][3]) * up_g8);
+          }
+        }
+      }
+      __syncthreads();
+      const int live = min(kw, spans);
+      for (int i = tid; i < kTile * 64; i += kThreads) {
+        const int r = i % 64;
+        if (r64 + r < rank) {
+          float sum = 0.f;
+          for (int w = 0; w < live; ++w) sum += part[w * kTile * 64 + i];
+          v_part[i / 64 * v_row + r64 + r] += sum;
+        }
+      }
+      __syncthreads();
+    }
+  }
+
+  // ---- the cluster's v
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int i = tid; i < kTile * v_row; i += kThreads) {
+    float sum = 0.f;
+    for (int b = 0; b < blocks; ++b) sum += cluster.map_shared_rank(v_part, b)[i];
+    v[i] = sum * scale;
+  }
+  cluster.sync();  // no block leaves before all have read
+
+  // ---- out = base + up v, K::unit rows a warp
+  const int token_g = g < n ? s_tokens[g] : -1, token_g8 = g + 8 < n ? s_tokens[g + 8] : -1;
+  float vs[2] = {1.f, 1.f};
+  if (K::f16) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float top = 0.f;
+      for (int r = t; r < rank; r += 4) top = fmaxf(top, fabsf(v[(g + 8 * h) * v_row + r]));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+      vs[h] = scale_to_two(top);
+    }
+  }
+  const float vi[2] = {1.f / vs[0], 1.f / vs[1]};
+#pragma unroll 1
+  for (int mu = m0 + warp * K::unit; mu < m1; mu += kWarps * K::unit) {
+    float acc[K::epc][4];
+#pragma unroll
+    for (int e = 0; e < K::epc; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[e][i] = 0.f;
+    // this lane's results: rows mu + (2t + i) epc + e of tokens g and g + 8
+    float base[K::epc][4];
+#pragma unroll
+    for (int e = 0; e < K::epc; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = mu + (2 * t + i % 2) * K::epc + e, tok = i < 2 ? token_g : token_g8;
+        base[e][i] = a.base.ptr && tok >= 0 && m < m1
+                         ? to_f32(static_cast<const T *>(a.base.ptr)[m * a.base.stride[0] + tok * a.base.stride[1]])
+                         : 0.f;
+      }
+    const int piece = mu + g * K::epc < s.out_row ? mu + g * K::epc : 0;
+    constexpr int R = K::f32 ? 2 : 4;  // rank rows of a lane in a step
+#pragma unroll 2
+    for (int r0 = 0; r0 < rank; r0 += K::step) {
+      uint4 w[R];
+      float va[2][R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int r = r0 + 2 * t + (i & 1) + (i & 2) * 4;
+        w[i] = __ldg(reinterpret_cast<const uint4 *>(up + (int64_t)min(r, rank - 1) * s.out_row + piece));  // beyond: v is zero
+        va[0][i] = v[g * v_row + r] * vi[0];
+        va[1][i] = v[(g + 8) * v_row + r] * vi[1];
+      }
+      uint32_t f[K::pv][4];
+      if (K::f32) {
+        f[0][0] = mma::tf32_head(va[0][0]), f[0][1] = mma::tf32_head(va[1][0]);
+        f[0][2] = mma::tf32_head(va[0][1]), f[0][3] = mma::tf32_head(va[1][1]);
+        f[K::pv - 1][0] = mma::tf32_tail(va[0][0]), f[K::pv - 1][1] = mma::tf32_tail(va[1][0]);
+        f[K::pv - 1][2] = mma::tf32_tail(va[0][1]), f[K::pv - 1][3] = mma::tf32_tail(va[1][1]);
+      } else {
+        uint32_t lo[K::pv][2], hi[K::pv][2];
+        split2<K::mode>(va[0][0], va[0][1], va[1][0], va[1][1], lo);
+        split2<K::mode>(va[0][R - 2], va[0][R - 1], va[1][R - 2], va[1][R - 1], hi);
+#pragma unroll
+        for (int p = 0; p < K::pv; ++p) f[p][0] = lo[p][0], f[p][1] = lo[p][1], f[p][2] = hi[p][0], f[p][3] = hi[p][1];
+      }
+#pragma unroll
+      for (int e = 0; e < K::epc; ++e) {
+        auto word = [&](int i) {
+          const int k = K::f32 ? e : e / 2;
+          return k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w;
+        };
+        if (K::f32) {
+          const float b0 = __uint_as_float(word(0)), b1 = __uint_as_float(word(1));
+#pragma unroll
+          for (int p = 0; p < K::pv; ++p)
+            mma::mma16<K::mode>(acc[e], f[p][0], f[p][1], f[p][2], f[p][3], mma::tf32_head(b0), mma::tf32_head(b1));
+          mma::mma16<K::mode>(acc[e], f[0][0], f[0][1], f[0][2], f[0][3], mma::tf32_tail(b0), mma::tf32_tail(b1));
+        } else {
+          const uint32_t sel = e % 2 ? 0x7632 : 0x5410;
+          const uint32_t b0 = __byte_perm(word(0), word(1), sel), b1 = __byte_perm(word(R - 2), word(R - 1), sel);
+#pragma unroll
+          for (int p = 0; p < K::pv; ++p) mma::mma16<K::mode>(acc[e], f[p][0], f[p][1], f[p][2], f[p][3], b0, b1);
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < K::epc; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = mu + (2 * t + i % 2) * K::epc + e, tok = i < 2 ? token_g : token_g8;
+        if (tok >= 0 && m < m1)
+          static_cast<T *>(a.out.ptr)[m * a.out.stride[0] + tok * a.out.stride[1]] =
+              from_f32<T>(fmaf(acc[e][i], vs[i / 2], base[e][i]));
+      }
+  }
+}
+
+// Sorts the tokens by adapter (those without one last) and cuts them into tiles; one block.  Tokens of 32 at a time
+// keep their order, so that neighbouring tokens of a prompt stay neighbours.
+__global__ void __launch_bounds__(1024) group_kernel(const __grid_constant__ SetView s, const int32_t *ids, int n, int *heads,
+                                                     int *tokens, Tile *tiles, int *n_tiles) {
+  __shared__ int s_a[32], s_b[32], s_tokens, s_tiles;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, bins = s.count + 1;
+  auto bin_of = [&](int i) {
+    const int id = ids[i];
+    if (id >= s.count) set_status(s.status, 10);
+    return id < 0 || id >= s.count || s.first[id + 1] == s.first[id] ? s.count : id;
+  };
+  for (int i = tid; i < bins; i += 1024) heads[i] = 0;
+  if (tid == 0) s_tokens = s_tiles = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += 1024) atomicAdd(&heads[bin_of(i)], 1);
+  __syncthreads();
+  // running sums of tokens and tiles over the bins
+  for (int b0 = 0; b0 < bins; b0 += 1024) {
+    const int b = b0 + tid, count = b < bins ? heads[b] : 0, cut = (count + kTile - 1) / kTile;
+    int x = count, y = cut;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int ux = __shfl_up_sync(~0u, x, d), uy = __shfl_up_sync(~0u, y, d);
+      if (lane >= d) x += ux, y += uy;
+    }
+    if (lane == 31) s_a[warp] = x, s_b[warp] = y;
+    __syncthreads();
+    int px = s_tokens, py = s_tiles, all = 0, cuts = 0;
+    for (int w = 0; w < 32; ++w) {
+      if (w < warp) px += s_a[w], py += s_b[w];
+      all += s_a[w], cuts += s_b[w];
+    }
+    const int first = px + x - count;
+    if (b < bins) heads[b] = first;
+    for (int k = 0; k < cut; ++k)
+      tiles[py + y - cut + k] = Tile{b == s.count ? -1 : b, first + k * kTile, min(kTile, count - k * kTile)};
+    __syncthreads();
+    if (tid == 0) s_tokens += all, s_tiles += cuts;
+    __syncthreads();
+  }
+  for (int i0 = 0; i0 < n; i0 += 1024) {
+    const int i = i0 + tid;
+    const int bin = i < n ? bin_of(i) : -1;
+    const uint32_t peers = __match_any_sync(~0u, bin);
+    const int leader = __ffs(peers) - 1;
+    int at = 0;
+    if (lane == leader && bin >= 0) at = atomicAdd(&heads[bin], __popc(peers));
+    at = __shfl_sync(~0u, at, leader);
+    if (bin >= 0) tokens[at + __popc(peers & ((1u << lane) - 1))] = i;
+  }
+  if (tid == 0) *n_tiles = s_tiles;
 }
 
 template <class F>
@@ -289,6 +707,37 @@ void with_types(int64_t rows, int64_t weights, F f) {
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
+// The scratch of a call with many tokens.
+struct Scratch {
+  int *n_tiles, *heads, *tokens;
+  Tile *tiles;
+  int64_t most_tiles;
+  size_t bytes;
+};
+Scratch scratch_of(const SetView &v, int64_t tokens, void *at) {
+  uint8_t *p = static_cast<uint8_t *>(at);
+  size_t used = 0;
+  auto take = [&](size_t n) {
+    uint8_t *q = p + used;
+    used += align256(n);
+    return q;
+  };
+  Scratch s;
+  s.most_tiles = tokens / kTile + std::min<int64_t>(v.count + 1, tokens);
+  s.n_tiles = reinterpret_cast<int *>(take(4));
+  s.heads = reinterpret_cast<int *>(take((v.count + 1) * sizeof(int)));
+  s.tokens = reinterpret_cast<int *>(take(tokens * sizeof(int)));
+  s.tiles = reinterpret_cast<Tile *>(take(s.most_tiles * sizeof(Tile)));
+  s.bytes = used;
+  return s;
+}
+
+// Shared memory of the tile kernel: x, the warps' parts of v (later v), the block's part of v.
+int tile_smem(int rank_max) {
+  const int v = kTile * ((rank_max + 15) / 16 * 16 + 4);
+  return 4 * (kTile * kXRow + std::max(kWarps * kTile * 64, v) + v);
+}
+
 }  // namespace
 
 struct sc_adapters {
@@ -307,6 +756,7 @@ int sc_adapters_create(int32_t device, int64_t in_features, int64_t out_features
   SC_SERVE_BEGIN
   require(out && ranks && down && down_ld && up && up_ld && scales, SC_ERR_ARG, "null argument");
   *out = nullptr;
+  require(device >= 0 && device < 64, SC_ERR_ARG, "bad device");
   require(count > 0 && count < (1 << 24), SC_ERR_ARG, "a set has 1 to 2^24 adapters");
   require(in_features > 0 && out_features > 0 && in_features < (1 << 24) && out_features < (1 << 24), SC_ERR_ARG,
           "features must be 1 to 2^24");
@@ -365,7 +815,7 @@ void sc_adapters_free(sc_adapters *s) { delete s; }
 int sc_adapters_workspace(const sc_adapters *s, int64_t tokens, int64_t *bytes) {
   SC_SERVE_BEGIN
   require(s && bytes && tokens >= 0, SC_ERR_ARG, "null argument or negative token count");
-  *bytes = tokens <= kFewTokens ? 0 : (int64_t)align256((size_t)tokens * s->view.rank_max * 4);
+  *bytes = tokens <= kFewTokens ? 0 : (int64_t)scratch_of(s->view, tokens, nullptr).bytes;
   SC_SERVE_END
 }
 
@@ -390,17 +840,40 @@ int sc_adapters_apply(sc_adapters *s, const sc_adapters_args *a, void *stream) {
           SC_ERR_ARG, "workspace missing, too small or not 16-byte aligned");
   DeviceGuard dg(s->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  float *v = static_cast<float *>(a->workspace);
   with_types(a->type, s->type, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
-    if (a->tokens <= kFewTokens) {
-      few_kernel<T, W><<<dim3(kCluster, (unsigned)a->tokens), kFewThreads, 0, st>>>(s->view, *a);
+    const bool few = a->tokens <= kFewTokens;
+    const Scratch sc = few ? Scratch{} : scratch_of(s->view, a->tokens, a->workspace);
+    const int64_t clusters = few ? a->tokens : sc.most_tiles;
+    require(clusters <= 65535, SC_ERR_UNSUPPORTED, "too many tokens in one call");
+    if (!few) group_kernel<<<1, 1024, 0, st>>>(s->view, a->ids, (int)a->tokens, sc.heads, sc.tokens, sc.tiles, sc.n_tiles);
+    // As many blocks a cluster as still run at once.  Few tokens: TODO blocks a SM by tokens; prompts: two.
+    int blocks = kMaxCluster;
+    while (blocks > 2 && clusters * blocks > (few ? 4 : 2) * 148) blocks /= 2;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = blocks;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks, (unsigned)clusters);
+    cfg.blockDim = dim3(few ? kFewThreads : kThreads);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (few) {
+      cuda_check(cudaLaunchKernelEx(&cfg, few_kernel<T, W>, s->view, *a), "launch adapters");
       return;
     }
-    const int64_t warps = a->tokens * s->view.rank_max, elems = a->tokens * s->view.out;
-    if (warps) shrink_kernel<decltype(t), decltype(w)><<<(unsigned)((warps + 7) / 8), 256, 0, st>>>(s->view, *a, v);
-    expand_kernel<decltype(t), decltype(w)><<<(unsigned)((elems + 255) / 256), 256, 0, st>>>(s->view, *a, v);
+    cfg.dynamicSmemBytes = tile_smem(s->view.rank_max);
+    auto kernel = tile_kernel<T, W>;
+    static std::atomic<uint64_t> ready{0};  // devices where the kernel may use this much shared memory
+    if (!(ready.load() >> s->device & 1)) {
+      cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem(kMaxRank)),
+                 "set shared memory size");
+      ready |= (uint64_t)1 << s->device;
+    }
+    cuda_check(cudaLaunchKernelEx(&cfg, kernel, s->view, *a, Sorted{sc.tiles, sc.tokens, sc.n_tiles}), "launch adapters");
   });
   cuda_check(cudaGetLastError(), "launch adapters");
   SC_SERVE_END

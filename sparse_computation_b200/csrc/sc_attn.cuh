@@ -41,17 +41,16 @@
 // keys, so results do not depend on the order of arrival.
 #pragma once
 
+#include "sc_mma.cuh"
 #include "sc_serve.h"
 
 namespace sc {
 namespace attn {
 
 using serve::to_f32;
+using namespace mma;
 
 constexpr int kQT = 8, kMaxWarps = 12, kWindow = 128;
-
-enum Mode { kTF32, kBF16, kBF16Wide, kBF16Wide4, kF16, kF16Wide };
-__host__ __device__ constexpr bool is_f16(int mode) { return mode == kF16 || mode == kF16Wide; }
 
 struct Params {
   sc_attn_args a;
@@ -141,47 +140,6 @@ __device__ __forceinline__ float4 ld_relaxed4(const float *p) {
   float4 v;
   asm volatile("ld.relaxed.gpu.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
   return v;
-}
-
-template <int MODE>
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1) {
-  if (MODE == kTF32)
-    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else if (is_f16(MODE))
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// The TF32 head of x: its upper 11 significant bits; x - head is exact.
-__device__ __forceinline__ uint32_t tf32_head(float x) { return __float_as_uint(x) & 0xffffe000u; }
-__device__ __forceinline__ uint32_t tf32_tail(float x) {
-  return __float_as_uint(x - __uint_as_float(__float_as_uint(x) & 0xffffe000u));
-}
-
-// Two floats as packed 16-bit values, and what the packing lost of them.
-template <int MODE>
-__device__ __forceinline__ uint32_t pack2(float &a, float &b) {
-  if (is_f16(MODE)) {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    a -= f.x;
-    b -= f.y;
-    return *reinterpret_cast<const uint32_t *>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    const float2 f = __bfloat1622float2(h);
-    a -= f.x;
-    b -= f.y;
-    return *reinterpret_cast<const uint32_t *>(&h);
-  }
 }
 
 // Four neighbouring outputs.  Out of line: it is not worth a copy at each of its uses.
@@ -605,15 +563,15 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
               const float k0 = __uint_as_float(kw[e]), k1 = __uint_as_float(kw[e + 1]);
-              mma<MODE>(s[nt][0], qh[e], ql[e], qh[e + 1], ql[e + 1], tf32_head(k0), tf32_head(k1));
-              mma<MODE>(s[nt][1], qh[e], ql[e], qh[e + 1], ql[e + 1], tf32_tail(k0), tf32_tail(k1));
+              mma16<MODE>(s[nt][0], qh[e], ql[e], qh[e + 1], ql[e + 1], tf32_head(k0), tf32_head(k1));
+              mma16<MODE>(s[nt][1], qh[e], ql[e], qh[e + 1], ql[e + 1], tf32_tail(k0), tf32_tail(k1));
             }
           } else {
-            mma<MODE>(s[nt][0], a0.x, a1.x, a0.y, a1.y, k.x, k.y);
-            mma<MODE>(s[nt][1], a0.z, a1.z, a0.w, a1.w, k.z, k.w);
+            mma16<MODE>(s[nt][0], a0.x, a1.x, a0.y, a1.y, k.x, k.y);
+            mma16<MODE>(s[nt][1], a0.z, a1.z, a0.w, a1.w, k.z, k.w);
             if (MODE == kBF16Wide) {
-              mma<MODE>(s[nt][0], q[C::parts - 1].x, 0, q[C::parts - 1].y, 0, k.x, k.y);
-              mma<MODE>(s[nt][1], q[C::parts - 1].z, 0, q[C::parts - 1].w, 0, k.z, k.w);
+              mma16<MODE>(s[nt][0], q[C::parts - 1].x, 0, q[C::parts - 1].y, 0, k.x, k.y);
+              mma16<MODE>(s[nt][1], q[C::parts - 1].z, 0, q[C::parts - 1].w, 0, k.z, k.w);
             }
           }
         }
@@ -692,15 +650,15 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
           for (int k = 0; k < PN; ++k) {
             if (C::f32) {
               const float v0 = __uint_as_float(word(2 * k)), v1 = __uint_as_float(word(2 * k + 1));
-              mma<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], tf32_head(v0), tf32_head(v1));
-              mma<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], tf32_tail(v0), tf32_tail(v1));
+              mma16<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], tf32_head(v0), tf32_head(v1));
+              mma16<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], tf32_tail(v0), tf32_tail(v1));
             } else {
               const uint32_t sel = e % 2 ? 0x7632 : 0x5410;
               constexpr int two = C::f32 ? 0 : 4;
               const uint32_t b0 = __byte_perm(word(two * k), word(two * k + 1 % (two + 1)), sel);
               const uint32_t b1 = __byte_perm(word(two * k + two / 2), word(two * k + two / 2 + 1 % (two + 1)), sel);
-              mma<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], b0, b1);
-              if (MODE == kBF16Wide) mma<MODE>(acc, p3[k][0], 0, p3[k][1], 0, b0, b1);
+              mma16<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], b0, b1);
+              if (MODE == kBF16Wide) mma16<MODE>(acc, p3[k][0], 0, p3[k][1], 0, b0, b1);
             }
           }
           float *oo = o[j * C::epc + e];

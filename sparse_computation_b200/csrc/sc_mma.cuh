@@ -1,0 +1,59 @@
+// Matrix instructions (mma.sync, 16 rows by 8 columns, fp32 sums) and the
+// splitting of fp32 operands into parts that they take.
+#pragma once
+
+#include <cstdint>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace sc {
+namespace mma {
+
+// Operand types; Wide: fp32 on one side, split into parts of the other side's type.
+enum Mode { kTF32, kBF16, kBF16Wide, kBF16Wide4, kF16, kF16Wide };
+__host__ __device__ constexpr bool is_f16(int mode) { return mode == kF16 || mode == kF16Wide; }
+
+template <int MODE>
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+  if (MODE == kTF32)
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else if (is_f16(MODE))
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The TF32 head of x: its upper 11 significant bits; x - head is exact.
+__device__ __forceinline__ uint32_t tf32_head(float x) { return __float_as_uint(x) & 0xffffe000u; }
+__device__ __forceinline__ uint32_t tf32_tail(float x) {
+  return __float_as_uint(x - __uint_as_float(__float_as_uint(x) & 0xffffe000u));
+}
+
+// Two floats as packed 16-bit values, and what the packing lost of them.
+template <int MODE>
+__device__ __forceinline__ uint32_t pack2(float &a, float &b) {
+  if (is_f16(MODE)) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    a -= f.x;
+    b -= f.y;
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const float2 f = __bfloat1622float2(h);
+    a -= f.x;
+    b -= f.y;
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+}
+
+}  // namespace mma
+}  // namespace sc
