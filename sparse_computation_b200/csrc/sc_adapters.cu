@@ -73,8 +73,9 @@ struct Eight {
   }
 };
 
-struct FewShared {
-  union {
+// 16-byte aligned: x and sums are read in fours.
+struct alignas(16) FewShared {
+  union alignas(16) {
     float x[kGroup][kFewChunk];           // this block's part of the tokens' x
     float sums[kGroup][kFewThreads * 8];  // parts of up v
   };
@@ -270,6 +271,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewBlocks) few_kernel(const __gr
       few_shrink<1>(sh, down + k, s.in_row, rank, wide);
     else if (n == 2)
       few_shrink<2>(sh, down + k, s.in_row, rank, wide);
+    else if (n == 3)
+      few_shrink<3>(sh, down + k, s.in_row, rank, wide);
     else
       few_shrink<kGroup>(sh, down + k, s.in_row, rank, wide);
     __syncthreads();
@@ -288,6 +291,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewBlocks) few_kernel(const __gr
     few_expand<1, T>(sh, a, up, s.out_row, rank, m0, m1 - m0);
   else if (n == 2)
     few_expand<2, T>(sh, a, up, s.out_row, rank, m0, m1 - m0);
+  else if (n == 3)
+    few_expand<3, T>(sh, a, up, s.out_row, rank, m0, m1 - m0);
   else
     few_expand<kGroup, T>(sh, a, up, s.out_row, rank, m0, m1 - m0);
 }
@@ -744,6 +749,7 @@ struct sc_adapters {
   int device = 0;
   int64_t type = 0;
   SetView view{};
+  int64_t mean_bytes = 0;  // of an adapter's weights
   DeviceBlock mem;
 };
 
@@ -806,6 +812,7 @@ int sc_adapters_create(int32_t device, int64_t in_features, int64_t out_features
   cuda_check(cudaStreamSynchronize(st), "stream synchronize");
   s->view = SetView{d_down,          d_up,        reinterpret_cast<int32_t *>(d_first), reinterpret_cast<float *>(d_scale),
                     in_features,     out_features, in_row, out_row, (int)count, (int)most, reinterpret_cast<int *>(d_status)};
+  s->mean_bytes = (int64_t)((b_down + b_up) / count);
   *out = s.release();
   SC_SERVE_END
 }
@@ -848,9 +855,15 @@ int sc_adapters_apply(sc_adapters *s, const sc_adapters_args *a, void *stream) {
     const int64_t clusters = few ? a->tokens : sc.most_tiles;
     require(clusters <= 65535, SC_ERR_UNSUPPORTED, "too many tokens in one call");
     if (!few) group_kernel<<<1, 1024, 0, st>>>(s->view, a->ids, (int)a->tokens, sc.heads, sc.tokens, sc.tiles, sc.n_tiles);
-    // As many blocks a cluster as still run at once.  Few tokens: TODO blocks a SM by tokens; prompts: two.
+    // Blocks a cluster.  Few tokens: eight, fewer while they would not all run at once (the clusters of tokens that lead
+    // no group come and go, but each costs its turn) and a block's share of an adapter stays below 32 KB: 4 x 148 blocks
+    // of 22 KB instead of 7 x 148 of 44 KB took 15.6 us instead of 22.4 (128 tokens, 100 adapters of 512 x 2048), but
+    // 38 us instead of 23 where they hold 147 and 74 KB (96 tokens, 40 adapters of 4096 x 4096).  Prompts: two a SM.
     int blocks = kMaxCluster;
-    while (blocks > 2 && clusters * blocks > (few ? 4 : 2) * 148) blocks /= 2;
+    if (few)
+      while (blocks > 2 && clusters * blocks > 4 * 148 && s->mean_bytes / blocks < 32 << 10) blocks /= 2;
+    else
+      while (blocks > 2 && clusters * blocks > 2 * 148) blocks /= 2;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = blocks;
