@@ -396,32 +396,68 @@ __global__ void __launch_bounds__(kThreads, 2)
                                                    i % lines * 128));
   }
   const int v_row = (rank + 15) / 16 * 16 + 4;  // floats; ranks up to a multiple of 16 are zeros
-  float *x_tile = smem, *part = smem + kTile * kXRow, *v_part = part + kWarps * kTile * 64;
+  float *part = smem + 2 * kTile * kXRow, *v_part = part + kWarps * kTile * 64;
   float *v = part;  // after the parts are added up
   for (int i = tid; i < kTile * v_row; i += kThreads) v_part[i] = 0.f;
 
-  // ---- v = down x over this block's columns, kChunk at a time
-  for (int k = k0; k < k1; k += kChunk) {
-    const int width = min(kChunk, k1 - k);
-    const bool by_token = a.x.stride[1] == 1;  // neighbouring threads on neighbouring tokens, else on neighbouring features
-    __syncthreads();
-#pragma unroll 1
-    for (int i0 = tid; i0 < kTile * kChunk; i0 += 8 * kThreads) {
-      float x[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int i = i0 + u * kThreads, row = by_token ? i % kTile : i / kChunk, col = by_token ? i / kTile : i % kChunk;
-        x[u] = row < n && col < width
-                   ? to_f32(static_cast<const T *>(a.x.ptr)[(k + col) * a.x.stride[0] + (int64_t)s_tokens[row] * a.x.stride[1]])
-                   : 0.f;
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int i = i0 + u * kThreads, row = by_token ? i % kTile : i / kChunk, col = by_token ? i / kTile : i % kChunk;
-        if (col < (width + kSpan - 1) / kSpan * kSpan) x_tile[row * kXRow + col] = x[u];
-      }
-      if ((by_token ? (i0 - tid + 8 * kThreads) / kTile : 0) >= (width + kSpan - 1) / kSpan * kSpan) break;
+  // base on its way to L2: rows m0.. of the tile's tokens
+  if (a.base.ptr) {
+    const bool by_token = a.base.stride[1] == 1;  // then the tokens of a row mostly share a line
+    const int per = by_token ? 1 : (m1 - m0 + 31) / 32, count = by_token ? m1 - m0 : per * n;
+    for (int i = tid; i < count; i += kThreads) {
+      const int64_t m = by_token ? m0 + i : min(m0 + i % per * 32, m1 - 1), tok = s_tokens[by_token ? 0 : i / per];
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const T *>(a.base.ptr) + m * a.base.stride[0] +
+                                                   tok * a.base.stride[1]));
     }
+  }
+
+  // ---- v = down x over this block's columns, kChunk at a time; x is asked for two chunks ahead
+  const bool by_token = a.x.stride[1] == 1;  // neighbouring threads on neighbouring tokens, else on neighbouring features
+  auto stage = [&](int chunk) {
+    const int k = k0 + chunk * kChunk, width = min(kChunk, k1 - k), wide = (width + kSpan - 1) / kSpan * kSpan;
+    float *to = smem + (chunk & 1) * (kTile * kXRow);
+    if (width > 0) {
+      // a thread keeps to a token (by_token: its columns are kThreads / kTile apart) or walks a token's columns; pointers
+      // move by additions only, as index arithmetic for each element took as long as the rest of the kernel
+      const T *x = static_cast<const T *>(a.x.ptr) + k * a.x.stride[0];
+      const int across = by_token ? kThreads / kTile : kThreads, rows = by_token ? 1 : kTile;
+      const int first = by_token ? tid / kTile : tid;
+      const int64_t step = across * a.x.stride[0];
+      for (int r = 0; r < rows; ++r) {
+        const int row = by_token ? tid % kTile : r;
+        const T *src = x + first * a.x.stride[0] + (row < n ? s_tokens[row] * a.x.stride[1] : 0);
+        float *dst = to + row * kXRow + first;
+        if (sizeof(T) == 4) {
+          uint32_t at = (uint32_t)__cvta_generic_to_shared(dst);
+#pragma unroll 4
+          for (int col = first; col < wide; col += across, src += step, at += across * 4) {
+            const bool in = row < n && col < width;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at), "l"(in ? src : x), "r"(in ? 4 : 0)
+                         : "memory");
+          }
+        } else {
+          for (int col0 = first; col0 < wide; col0 += 8 * across, src += 8 * step, dst += 8 * across) {
+            T v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              if (row < n && col0 + u * across < width) v[u] = src[u * step];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const int col = col0 + u * across;
+              if (col < wide) dst[u * across] = row < n && col < width ? to_f32(v[u]) : 0.f;
+            }
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;");
+  };
+  stage(0);
+  stage(1);
+  for (int k = k0, chunk = 0; k < k1; k += kChunk, ++chunk) {
+    const int width = min(kChunk, k1 - k);
+    float *x_tile = smem + (chunk & 1) * (kTile * kXRow);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncthreads();
     // warps: kw of them along the columns, kSpan each, the others along the ranks
     const int spans = (width + kSpan - 1) / kSpan, kw = spans > 4 ? 8 : spans > 2 ? 4 : spans;
@@ -538,7 +574,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       __syncthreads();
     }
+    stage(chunk + 2);  // every warp has its fragments of this chunk
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 
   // ---- the cluster's v
   cg::cluster_group cluster = cg::this_cluster();
@@ -571,17 +609,17 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int e = 0; e < K::epc; ++e)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[e][i] = 0.f;
-    // this lane's results: rows mu + (2t + i) epc + e of tokens g and g + 8
-    float base[K::epc][4];
+    // this lane's results: the 2 epc rows from mu + 2t epc on of tokens g and g + 8
+    const int row0 = mu + 2 * t * K::epc;
+    float base[2][2 * K::epc];
 #pragma unroll
-    for (int e = 0; e < K::epc; ++e)
+    for (int h = 0; h < 2; ++h) {
+      const int tok = h ? token_g8 : token_g;
+      const T *p = static_cast<const T *>(a.base.ptr) + row0 * a.base.stride[0] + tok * a.base.stride[1];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int m = mu + (2 * t + i % 2) * K::epc + e, tok = i < 2 ? token_g : token_g8;
-        base[e][i] = a.base.ptr && tok >= 0 && m < m1
-                         ? to_f32(static_cast<const T *>(a.base.ptr)[m * a.base.stride[0] + tok * a.base.stride[1]])
-                         : 0.f;
-      }
+      for (int r = 0; r < 2 * K::epc; ++r, p += a.base.stride[0])
+        base[h][r] = a.base.ptr && tok >= 0 && row0 + r < m1 ? to_f32(*p) : 0.f;
+    }
     const int piece = mu + g * K::epc < s.out_row ? mu + g * K::epc : 0;
     constexpr int R = K::f32 ? 2 : 4;  // rank rows of a lane in a step
 #pragma unroll 2
@@ -629,14 +667,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
 #pragma unroll
-    for (int e = 0; e < K::epc; ++e)
+    for (int h = 0; h < 2; ++h) {
+      const int tok = h ? token_g8 : token_g;
+      T *p = static_cast<T *>(a.out.ptr) + row0 * a.out.stride[0] + tok * a.out.stride[1];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int m = mu + (2 * t + i % 2) * K::epc + e, tok = i < 2 ? token_g : token_g8;
-        if (tok >= 0 && m < m1)
-          static_cast<T *>(a.out.ptr)[m * a.out.stride[0] + tok * a.out.stride[1]] =
-              from_f32<T>(fmaf(acc[e][i], vs[i / 2], base[e][i]));
-      }
+      for (int r = 0; r < 2 * K::epc; ++r, p += a.out.stride[0])
+        if (tok >= 0 && row0 + r < m1) *p = from_f32<T>(fmaf(acc[r % K::epc][2 * h + r / K::epc], vs[h], base[h][r]));
+    }
   }
 }
 
@@ -644,8 +681,10 @@ __global__ void __launch_bounds__(kThreads, 2)
 // keep their order, so that neighbouring tokens of a prompt stay neighbours.
 __global__ void __launch_bounds__(1024) group_kernel(const __grid_constant__ SetView s, const int32_t *ids, int n, int *heads,
                                                      int *tokens, Tile *tiles, int *n_tiles) {
-  __shared__ int s_a[32], s_b[32], s_tokens, s_tiles;
+  constexpr int kBins = 2048;  // so many counters fit shared memory
+  __shared__ int s_a[32], s_b[32], s_tokens, s_tiles, s_heads[kBins];
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, bins = s.count + 1;
+  if (bins <= kBins) heads = s_heads;
   auto bin_of = [&](int i) {
     const int id = ids[i];
     if (id >= s.count) set_status(s.status, 10);
@@ -666,11 +705,9 @@ __global__ void __launch_bounds__(1024) group_kernel(const __grid_constant__ Set
     }
     if (lane == 31) s_a[warp] = x, s_b[warp] = y;
     __syncthreads();
-    int px = s_tokens, py = s_tiles, all = 0, cuts = 0;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) px += s_a[w], py += s_b[w];
-      all += s_a[w], cuts += s_b[w];
-    }
+    const int all = __reduce_add_sync(~0u, s_a[lane]), cuts = __reduce_add_sync(~0u, s_b[lane]);
+    const int px = s_tokens + __reduce_add_sync(~0u, lane < warp ? s_a[lane] : 0);
+    const int py = s_tiles + __reduce_add_sync(~0u, lane < warp ? s_b[lane] : 0);
     const int first = px + x - count;
     if (b < bins) heads[b] = first;
     for (int k = 0; k < cut; ++k)
@@ -740,7 +777,7 @@ Scratch scratch_of(const SetView &v, int64_t tokens, void *at) {
 // Shared memory of the tile kernel: x, the warps' parts of v (later v), the block's part of v.
 int tile_smem(int rank_max) {
   const int v = kTile * ((rank_max + 15) / 16 * 16 + 4);
-  return 4 * (kTile * kXRow + std::max(kWarps * kTile * 64, v) + v);
+  return 4 * (2 * kTile * kXRow + std::max(kWarps * kTile * 64, v) + v);
 }
 
 }  // namespace
