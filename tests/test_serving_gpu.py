@@ -472,3 +472,92 @@ def test_decoding_steps_of_a_pruned_layer(cuda):
         assert (y - want).abs().max() <= 4 * 110 * 2.0 ** -24 * 20 * want.abs().max()
     cache.check()
     attention.check()
+
+
+# ------------------------------------------- adapters of many tokens -----
+
+MANY = [
+    # types, in, out, ranks, tokens of each adapter and without one (last), token-major, mixed
+    (TYPE_PAIRS[0], 5000, 300, [9, 40, 17], [700, 300, 400, 100], False, False),  # five chunks of columns a block
+    (TYPE_PAIRS[1], 5000, 300, [9, 40, 17], [700, 300, 400, 100], True, True),
+    (TYPE_PAIRS[2], 700, 1100, [200, 70], [200, 150, 3], False, False),  # more than 64 ranks
+    (TYPE_PAIRS[3], 576, 200, [256, 1, 0, 65], [100, 90, 80, 70, 30], True, False),
+    (TYPE_PAIRS[4], 520, 4000, [33, 64], [257, 0, 0], False, True),
+    (TYPE_PAIRS[5], 130, 70, [8], [300, 5], True, True),
+    (TYPE_PAIRS[1], 5000, 90, [12, 30], [3, 2, 1], False, True),  # few tokens, two chunks of columns a block
+]
+
+
+@pytest.mark.parametrize("types,k,m,ranks,counts,token_major,mixed", MANY)
+def test_adapters_many_tokens(cuda, types, k, m, ranks, counts, token_major, mixed):
+    gen = torch.Generator().manual_seed(12)
+    down, up, scales = adapter_set(gen, types, k, m, ranks)
+    ids = torch.tensor([i if i < len(ranks) else -1 for i, c in enumerate(counts) for _ in range(c)], dtype=torch.int32)
+    if mixed:
+        ids = ids[torch.randperm(len(ids), generator=gen)]
+    n = len(ids)
+    x, base = randn(gen, k, n, dtype=types[0]), randn(gen, m, n, dtype=types[0])
+    turn = (lambda y: y.t().contiguous().cuda().t()) if token_major else (lambda y: y.cuda())
+    s = sc.LowRankAdapters([a.cuda() for a in down], [b.cuda() for b in up], scales)
+    got = s.apply(turn(x), ids.cuda(), base=turn(base))
+    s.check()
+    want, tol = ref.adapters(x, ids, down, up, scales, base, types[0])
+    assert ((got.cpu().double() - want).abs() <= tol).all()
+    assert torch.equal(got, s.apply(turn(x), ids.cuda(), base=turn(base)))
+
+
+@pytest.mark.parametrize("tokens", [200, 600])
+def test_adapters_many_adapters(cuda, tokens):
+    """More adapters than a sorting block counts in shared memory, most of them unused; ids beyond the set are none."""
+    gen = torch.Generator().manual_seed(13)
+    count = 2100
+    down = [randn(gen, 1 + i % 3, 24) for i in range(count)]
+    up = [randn(gen, 40, 1 + i % 3) for i in range(count)]
+    s = sc.LowRankAdapters([a.cuda() for a in down], [b.cuda() for b in up], [0.5] * count)
+    ids = torch.randint(-1, count, (tokens,), generator=gen).int()
+    ids[7], ids[8] = 2099, 2100
+    x = randn(gen, 24, tokens)
+    got = s.apply(x.cuda(), ids.cuda())
+    assert s.status() == 10
+    want, tol = ref.adapters(x, ids, down, up, [0.5] * count, None, F32)
+    assert ((got.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("types", [TYPE_PAIRS[0], TYPE_PAIRS[1], TYPE_PAIRS[3], TYPE_PAIRS[4]])
+def test_attend_more_sequences_than_threads(cuda, types):
+    """The scan over the lengths takes several rounds; empty, tiny and longer sequences alternate."""
+    lens = [(i * 37) % 50 if i % 3 else (i % 2) for i in range(900)]
+    plan, q, table, sl, want = attend_case(types, 1, 2, 32, 16, 0, "tokens", "heads", lens)
+    close(*plan.attend(q, table, sl, return_lse=True), want)
+
+
+@pytest.mark.parametrize("page", [1, 2, 3, 8, 16, 17, 32, 100])
+def test_attend_page_sizes(cuda, page):
+    plan, q, table, sl, want = attend_case(TYPE_PAIRS[1], 2, 6, 64, page, 0, "tokens", "slots", [1, 31, 257, 1000])
+    close(*plan.attend(q, table, sl, return_lse=True), want)
+
+
+@pytest.mark.parametrize("t", [1, 3, 5, 9, 17, 40, 700])
+@pytest.mark.parametrize("layout", ["tokens", "features"])
+def test_append_token_counts(cuda, t, layout):
+    gen = torch.Generator().manual_seed(14)
+    h, d, page = 2, 64, 16
+    k, v, q = (randn(gen, t, n, d, dtype=BF16) for n in (h, h, 4))
+    pages = -(-t // page)
+    cache = sc.PagedKVCache.allocate(pages + 1, page, h, d, BF16)
+    cos, sin = tables(16)
+    pos = torch.arange(t, dtype=torch.int32)
+    table = torch.randperm(pages + 1, generator=gen)[:pages].int().view(1, -1)
+    got = cache.append(rows(k, layout), rows(v, layout), pos.cuda(), table.cuda(), torch.zeros(t, dtype=torch.int32).cuda(),
+                       rope=sc.RotaryTable(cos.cuda(), sin.cuda()), q=rows(q, layout))
+    cache.check()
+    for given, out in ((q, got.cpu()), (k, cache.k.cpu()[table[0].long()].transpose(1, 2).reshape(-1, h, d)[:t])):
+        want, mag = ref.rotate(given, pos, cos, sin, False)
+        assert ((out.double() - want).abs() <= 2.0 ** -22 * mag + ref.rounding(want, BF16) * (1 + 2.0 ** -6)).all()
+    assert torch.equal(cache.v.cpu()[table[0].long()].transpose(1, 2).reshape(-1, h, d)[:t], v)
+
+
+def test_decode_demo(cuda, capsys):
+    from sparse_computation_b200 import decode_demo
+    assert decode_demo.main(["--requests", "4", "--steps", "6", "--layers", "2", "--page", "4"]) > 0
+    assert "4 requests, 2 layers, bf16 cache" in capsys.readouterr().out
