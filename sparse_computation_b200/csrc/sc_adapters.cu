@@ -54,8 +54,8 @@ __global__ void pack_rows(const W *src, int64_t row_stride, int64_t col_stride, 
 // then each block makes its part of the rows of up v.  One launch, no scratch
 // memory.  Bound by latency (a chain of ids, weights, two cluster barriers,
 // weights) and fp32 instructions; the tensor-core tiles below have twice the
-// fixed cost: 128 tokens of 100 adapters of 512 x 2048 take 14.3 us here, 28.6
-// there.
+// fixed cost: 128 tokens of 100 adapters of 512 x 2048 in bf16 take 15.4 us
+// here, 28.6 there; 96 tokens of 40 adapters of 4096 x 4096 22.7 and 33.3.
 constexpr int kFewTokens = 256, kGroup = 4, kFewChunk = 512, kFewThreads = 256, kFewBlocks = 3;
 
 // Eight weights, as they lie.
@@ -311,13 +311,13 @@ __global__ void __launch_bounds__(kFewThreads, kFewBlocks) few_kernel(const __gr
 // result): of `down`, piece t + 4j of rank row g; of `up` (stored transposed),
 // the piece at rows 8g.. of ranks 2t, 2t+1 (+8).  What a 16-bit operand loses
 // of x and v goes into further parts, one instruction each (two TF32 parts on
-// both sides for fp32 weights), fp16 parts scaled by a power of two.  The same
-// with fp32 instructions took 22.5 us for 96 tokens of 40 adapters of
-// 4096 x 4096, bound by instructions; this takes TODO.
+// both sides for fp32 weights), fp16 parts scaled by a power of two.
 //
-// A block sorts the tokens by adapter first (group_kernel); tokens without one
-// are copied.  Bound by x and out at best, at present by instructions and the
-// barriers between the phases of a tile.
+// A block sorts the tokens by adapter first (group_kernel, 7 us for 2049
+// tokens); tokens without one are copied.  x and out bound it at best; at
+// present the latencies between the phases of a tile do, two blocks a SM:
+// 2049 fp32 tokens of 6 adapters, 2048 x 2048 in fp16, 55.9 us (one warp per
+// token and rank row, then one thread per result: 387).
 constexpr int kMaxCluster = 8, kTile = 16, kChunk = 512, kThreads = 256, kWarps = kThreads / 32;
 constexpr int kXRow = kChunk + 4, kSpan = 64;  // floats of a token's chunk in shared memory; columns of a warp
 

@@ -25,9 +25,11 @@
 // memory straight into the registers that feed the matrix instructions: the
 // next K is asked for as soon as the scores are done, the next V after the
 // product with P.  At 8 KB a warp step and 12 warps a SM that is 48-96 KB in
-// flight, more than latency times bandwidth asks for.  (Through cp.async and
-// shared memory, 16 warps: 147 us against 96 at 131071 keys, 8 kv heads of
-// 128, bf16; the 16 further shared-memory loads a step were the bound.)
+// flight, more than latency times bandwidth asks for.  A version with 16 warps
+// that went through cp.async and shared memory took 147 us at 131071 keys (8
+// kv heads of 128, bf16), a fifth of it in a slower join; this takes 92, 5.8
+// TB/s.  Row addresses are computed where they are needed: handing them round
+// by shuffles cost a fifth of the loop's speed.
 //
 // Work.  All (sequence, kv head, query tile) segments are cut into steps of
 // `keys` keys and laid end to end.  Every block takes one equal, contiguous
@@ -39,6 +41,12 @@
 // goes into a record in the workspace, and the last of its blocks to arrive
 // adds the records up.  Pieces and records are added in the order of the
 // keys, so results do not depend on the order of arrival.
+//
+// What is left over the read: the scan, the first loads, and the two joins, 5
+// to 10 us in all, most of it fetching code that each block runs once (25
+// cycles an instruction while the memory is busy).  128 fp32 requests of 16 to
+// 1024 keys, 8 heads of 64: 40 us against 19 for the bytes; 32 requests of 100
+// to 8192 keys, 32 / 8 heads of 128, fp32 queries over bf16: 65 against 39.
 #pragma once
 
 #include "sc_mma.cuh"

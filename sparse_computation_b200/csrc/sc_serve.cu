@@ -141,39 +141,59 @@ struct Divider {
 
 // Token-major activations (the heads of a token contiguous): a warp takes a
 // token, or 1/p.parts of it, so that position, page and rotation row are its
-// own scalars, and walks the heads in jobs of eight dims (with their eight
-// partners in the half style), BATCH of them in flight.  Bound by memory, but
-// at 16 bits the instructions of a job count as much: index computations of
-// one flat job list over all tokens took 20 us for 4099 tokens, against TODO.
+// own scalars.  It walks the heads of v, k and q in jobs of eight dims (with
+// their eight partners in the half style), and asks for the first jobs of all
+// three before the place of the token is known.  Bound by memory latency and,
+// at 16 bits, by the instructions of a job: walking v, k and q one after the
+// other took 16.3 us for 4099 tokens of 20 + 2 x 4 heads of 80 in bf16 (one
+// thread per pair 45.0), this 13.9: 2.7 TB/s.
 struct RowJobs {
   Divider jobs;  // of a head
   int half;      // distance of partners, 0: none
 };
 
-template <class T, class C, int BATCH, bool POOL>
-__device__ __forceinline__ void walk_heads(const T *src, C *dst, int64_t dst_head, const RowJobs &r, int heads, int rotary,
-                                           const float *cos, const float *sin, bool rope4, bool zero, int first, int step) {
-  const int n = heads * (int)r.jobs.by, D = (int)r.jobs.by * 8 + r.half;
-  for (int j0 = first; j0 < n; j0 += BATCH * step) {
-    Eight<T> u[BATCH], w[BATCH];
-    int d[BATCH], head[BATCH];
+struct Turn {  // the rotation of a token
+  const float *cos, *sin;
+  int rotary;  // 0: none
+  bool four;   // rows can be read in fours
+};
+
+// BATCH jobs of one lane, `step` apart.
+template <class T, int BATCH>
+struct HeadJobs {
+  Eight<T> u[BATCH], w[BATCH];
+
+  __device__ __forceinline__ void load(const T *src, const RowJobs &r, int heads, int first, int step) {
+    const int n = heads * (int)r.jobs.by, D = (int)r.jobs.by * 8 + r.half;
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
-      const int j = j0 + i * step;
-      head[i] = (int)r.jobs(j);
-      d[i] = (j - head[i] * (int)r.jobs.by) * 8;
-      if (d[i] >= r.half) d[i] += r.half;  // the partners' eights go with the first ones
+      const int j = first + i * step;
       if (j < n) {
-        u[i].load(src + head[i] * D + d[i]);
-        if (d[i] < r.half) w[i].load(src + head[i] * D + d[i] + r.half);
+        const int head = (int)r.jobs(j);
+        int d = (j - head * (int)r.jobs.by) * 8;
+        if (d >= r.half) d += r.half;  // the partners' eights go with the first ones
+        const T *p = src + head * D + d;
+        u[i].load(p);
+        if (d < r.half) w[i].load(p + r.half);
       }
     }
+  }
+
+  // dst_head 0: heads lie as in the source
+  template <class C>
+  __device__ __forceinline__ void finish(C *dst, int64_t dst_head, const RowJobs &r, int heads, const Turn &turn, bool zero, int first,
+                                         int step) {
+    const int n = heads * (int)r.jobs.by, D = (int)r.jobs.by * 8 + r.half;
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
-      if (j0 + i * step >= n) break;
-      C *y = dst + (POOL ? head[i] * dst_head : head[i] * D) + d[i];
-      const bool two = d[i] < r.half;
-      if (std::is_same<T, C>::value && d[i] >= rotary && !zero) {  // the bits move as they are
+      const int j = first + i * step;
+      if (j >= n) break;
+      const int head = (int)r.jobs(j);
+      int d = (j - head * (int)r.jobs.by) * 8;
+      if (d >= r.half) d += r.half;
+      const bool two = d < r.half;
+      C *y = dst + (dst_head ? head * dst_head : head * D) + d;
+      if (std::is_same<T, C>::value && d >= turn.rotary && !zero) {  // the bits move as they are
         u[i].store(reinterpret_cast<T *>(y));
         if (two) w[i].store(reinterpret_cast<T *>(y + r.half));
         continue;
@@ -181,13 +201,13 @@ __device__ __forceinline__ void walk_heads(const T *src, C *dst, int64_t dst_hea
       float x[8], z[8] = {};
       u[i].get(x);
       if (two) w[i].get(z);
-      if (d[i] < rotary) {
-        const float *cp = cos + (r.half ? d[i] : d[i] / 2), *sp = sin + (r.half ? d[i] : d[i] / 2);
+      if (d < turn.rotary) {
+        const float *cp = turn.cos + (r.half ? d : d / 2), *sp = turn.sin + (r.half ? d : d / 2);
         float c[8], s[8];
 #pragma unroll
         for (int e = 0; e < 8; e += 4)
           if (e == 0 || r.half) {
-            if (rope4) {
+            if (turn.four) {
               *reinterpret_cast<float4 *>(c + e) = *reinterpret_cast<const float4 *>(cp + e);
               *reinterpret_cast<float4 *>(s + e) = *reinterpret_cast<const float4 *>(sp + e);
             } else {
@@ -223,37 +243,56 @@ __device__ __forceinline__ void walk_heads(const T *src, C *dst, int64_t dst_hea
       }
     }
   }
-}
+};
 
 template <class T, class C>
-__global__ void __launch_bounds__(128) append_rows_kernel(const __grid_constant__ AppendParams p, const __grid_constant__ RowJobs turned,
-                                                          const __grid_constant__ RowJobs plain, int rope4) {
-  constexpr int B = sizeof(T) == 4 ? 2 : 4;
+__global__ void __launch_bounds__(128, 4) append_rows_kernel(const __grid_constant__ AppendParams p,
+                                                             const __grid_constant__ RowJobs turned,
+                                                             const __grid_constant__ RowJobs plain, int rope4) {
+  constexpr int BK = sizeof(T) == 4 ? 1 : 2, BQ = sizeof(T) == 4 ? 2 : 4;
   const sc_kv_append_args &a = p.a;
   const int64_t t = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32;
   if (t >= a.tokens) return;
+  const int first = blockIdx.y * 32 + threadIdx.x % 32, step = 32 * p.parts, hk = (int)p.pool.kv_heads;
+  const int hq = a.q.ptr ? (int)a.q_heads : 0;
+  const T *sv = static_cast<const T *>(a.v.ptr) + t * a.v.stride[0], *sk = static_cast<const T *>(a.k.ptr) + t * a.k.stride[0];
+  const T *sq = static_cast<const T *>(a.q.ptr) + t * a.q.stride[0];
+  HeadJobs<T, BK> v, k;
+  HeadJobs<T, BQ> q;
+  v.load(sv, plain, hk, first, step);
+  k.load(sk, turned, hk, first, step);
+  q.load(sq, turned, hq, first, step);
   int pos, page, slot;
   token_place(p, t, pos, page, slot);
-  const int first = blockIdx.y * 32 + threadIdx.x % 32, step = 32 * p.parts;
-  const int rotary = a.cos && page >= 0 ? (int)a.rotary : 0, hk = (int)p.pool.kv_heads;
-  const float *cos = a.cos + pos * a.rope_stride, *sin = a.sin + pos * a.rope_stride;
+  const Turn none{nullptr, nullptr, 0, false};
+  const Turn turn{a.cos + pos * a.rope_stride, a.sin + pos * a.rope_stride, a.cos && page >= 0 ? (int)a.rotary : 0, rope4 != 0};
   if (page >= 0) {
-    walk_heads<T, C, B, true>(static_cast<const T *>(a.v.ptr) + t * a.v.stride[0],
-                              static_cast<C *>(p.pool.v) + page * p.pool.v_stride[0] + slot * p.pool.v_stride[2],
-                              p.pool.v_stride[1], plain, hk, 0, cos, sin, false, false, first, step);
-    walk_heads<T, C, B, true>(static_cast<const T *>(a.k.ptr) + t * a.k.stride[0],
-                              static_cast<C *>(p.pool.k) + page * p.pool.k_stride[0] + slot * p.pool.k_stride[2],
-                              p.pool.k_stride[1], turned, hk, rotary, cos, sin, rope4, false, first, step);
+    C *dv = static_cast<C *>(p.pool.v) + page * p.pool.v_stride[0] + slot * p.pool.v_stride[2];
+    C *dk = static_cast<C *>(p.pool.k) + page * p.pool.k_stride[0] + slot * p.pool.k_stride[2];
+    const int64_t vh = hk > 1 ? p.pool.v_stride[1] : 0, kh = hk > 1 ? p.pool.k_stride[1] : 0;
+    v.finish(dv, vh, plain, hk, none, false, first, step);
+    k.finish(dk, kh, turned, hk, turn, false, first, step);
+#pragma unroll 1
+    for (int j = first + BK * step; j < hk * (int)plain.jobs.by; j += BK * step) {
+      v.load(sv, plain, hk, j, step);
+      k.load(sk, turned, hk, j, step);
+      v.finish(dv, vh, plain, hk, none, false, j, step);
+      k.finish(dk, kh, turned, hk, turn, false, j, step);
+    }
   }
-  if (a.q.ptr)
-    walk_heads<T, T, B, false>(static_cast<const T *>(a.q.ptr) + t * a.q.stride[0],
-                               static_cast<T *>(a.q_out.ptr) + t * a.q_out.stride[0], 0, turned, (int)a.q_heads, rotary, cos,
-                               sin, rope4, page < 0, first, step);
+  T *dq = static_cast<T *>(a.q_out.ptr) + t * a.q_out.stride[0];
+  for (int j = first; j < hq * (int)turned.jobs.by; j += BQ * step) {
+    if (j != first) q.load(sq, turned, hq, j, step);
+    q.finish(dq, 0, turned, hq, turn, page < 0, j, step);
+  }
 }
 
 // Feature-major activations, as a product leaves them (tokens contiguous): a
 // block takes one head of 2^p.tile_bits tokens, reads it along the tokens,
 // turns it in shared memory and writes it along the dims, two to a thread.
+// Bound by the chain of latencies (position, page entry, rotation row, store)
+// at decoding sizes: 128 tokens of 32 + 2 x 8 heads of 128, fp32 into bf16,
+// 6.9 us against 0.9 for their bytes; 4 tokens of 3 x 8 heads of 64 2.6 us.
 template <class T, class C>
 __global__ void __launch_bounds__(256) append_columns_kernel(const __grid_constant__ AppendParams p) {
   const sc_kv_append_args &a = p.a;
