@@ -116,7 +116,7 @@ int sc_attn_decode(sc_attn *p, const sc_attn_args *a, void *stream) {
   // the most steps that these lengths can have; the true number is known on the device only
   int64_t keys = std::min<int64_t>(a->table_cols, INT32_MAX / p->pool.page_size) * p->pool.page_size;
   if (p->window) keys = std::min(keys, p->window + 15);
-  const int64_t per_seq = std::max<int64_t>(1, (keys + v.keys - 1) / v.keys) + kSwitch, units = p->pool.kv_heads * p->qtiles;
+  const int64_t per_seq = std::max<int64_t>(1, (keys + v.keys - 1) / v.keys) + v.change, units = p->pool.kv_heads * p->qtiles;
   // places are counted in 32 bits, and a block's run may end one run beyond the last
   require(per_seq * a->seqs * units < INT32_MAX / 2, SC_ERR_UNSUPPORTED,
           "the page table names more keys than one call can take");

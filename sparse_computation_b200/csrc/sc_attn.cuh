@@ -45,8 +45,8 @@
 // What is left over the read: the scan, the first loads, and the two joins, 5
 // to 10 us in all, most of it fetching code that each block runs once (25
 // cycles an instruction while the memory is busy).  128 fp32 requests of 16 to
-// 1024 keys, 8 heads of 64: 40 us against 19 for the bytes; 32 requests of 100
-// to 8192 keys, 32 / 8 heads of 128, fp32 queries over bf16: 65 against 39.
+// 1024 keys, 8 heads of 64: 39 us against 19 for the bytes; 32 requests of 100
+// to 8192 keys, 32 / 8 heads of 128, fp32 queries over bf16: 63 against 39.
 #pragma once
 
 #include "sc_mma.cuh"
@@ -80,7 +80,7 @@ struct Params {
 // One instantiation of the kernel and what its launch needs.
 struct Variant {
   void (*kernel)(Params);
-  int warps, smem, keys, piece;
+  int warps, smem, keys, piece, change;
 };
 
 // The instantiation for a head_dim, made ready on the current device.
@@ -99,6 +99,11 @@ struct Cfg {
   static constexpr int keys = NT * 8, sub = keys < 16 ? keys : 16;
   static constexpr int q_row = KJ * parts * 64;              // bytes of one query row in fragment order
   static constexpr int max_warps = DP > 128 ? 8 : kMaxWarps;  // by the registers of a step
+  // Segments are laid end to end with this many places after each that hold no keys: they stand for what changing to
+  // another segment costs a warp (its query, its pages, its result) in steps.  us of 128 fp32 requests / of the ragged
+  // bf16 batch / of windows over fp16: 38.6 69.7 28.7 with 1, 39.9 65.5 26.4 with 2, 40.8 62.7 26.1 with 3, 42.1 61.9
+  // 26.9 with 4.
+  static constexpr int change = f32 ? 1 : 3;
   static constexpr bool ahead = DP <= 128;                   // registers suffice to load K a phase ahead
   static constexpr int o_row = DP + 4;                       // floats; the pad spreads rows over the banks
   static constexpr int piece = kQT * o_row + 2 * kQT;        // O | m | l
@@ -191,11 +196,6 @@ __device__ __forceinline__ int page_of(const Params &p, int key) {
 
 __device__ __forceinline__ float lse_of(float ref, float sum) { return (ref + log2f(sum)) * 0.69314718055994531f; }
 
-// Segments are laid end to end with kSwitch places after each that hold no
-// keys: they stand for what changing to another segment costs a warp (its
-// query, its pages, its result) in steps.
-constexpr int kSwitch = 2;
-
 // A boundary between two blocks' runs: the place that an equal cut gives,
 // moved to an end of its segment when that is near, which saves a join, or
 // when no keys are left there.
@@ -203,9 +203,10 @@ struct Cut {
   int at, seq_begin, seg_begin, seg_end, seq;
 };
 
+template <int CHANGE>
 __device__ __forceinline__ int snapped(int b, int x, int y, int near) {
   const int lo = b - x, hi = y - b;
-  return lo <= near && lo <= hi ? x : hi <= near || hi <= kSwitch ? y : b;
+  return lo <= near && lo <= hi ? x : hi <= near || hi <= CHANGE ? y : b;
 }
 
 template <int MODE, int DP, bool FULL>
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
   // ---- this block's run: a scan over the sequences, blockDim of them at a time
   auto places_of = [&](int s) {  // of one of its segments
     const int n = s < seqs ? span_of<C::keys>(p, s).steps : 0;
-    return n ? n + kSwitch : 0;
+    return n ? n + C::change : 0;
   };
   int n = places_of(tid), more = 0;
 #pragma unroll 1
@@ -251,6 +252,8 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
   int before = sum_of(s_scan, warp), chunk = sum_of(s_scan, W);
   const int total = (chunk + sum_of(s_more, W)) * units;
   const int per = max((int)((total + gridDim.x - 1) / gridDim.x), p.min_run);
+  // A join costs about what a block's eighth does, or half a step of every warp: with a quarter of either the smallest
+  // batch took 14 us instead of 11.4, with twice the eighth the ragged one 66.8 instead of 62.6.
   const int near = max(per / 8, min(per, W) / 2);
   const int nominal0 = per * blockIdx.x, nominal1 = nominal0 + per;
   if (nominal0 >= total) return;
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
       const int b = k ? nominal1 : nominal0;
       if (b >= from && b < to) {
         const int x = from + (b - from) / n * n;
-        s_cut[k] = Cut{snapped(b, x, x + n, near), from, x, x + n, base + tid};
+        s_cut[k] = Cut{snapped<C::change>(b, x, x + n, near), from, x, x + n, base + tid};
       }
     }
     base += blockDim.x;
@@ -304,12 +307,12 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
 #pragma unroll 1
     for (;;) {
 #pragma unroll 1
-      while (sp.steps == 0 || at >= seq_begin + (sp.steps + kSwitch) * units) {  // next sequence with keys
+      while (sp.steps == 0 || at >= seq_begin + (sp.steps + C::change) * units) {  // next sequence with keys
         if (at >= we) return;
-        if (sp.steps) seq_begin += (sp.steps + kSwitch) * units;
+        if (sp.steps) seq_begin += (sp.steps + C::change) * units;
         sp = span_of<C::keys>(p, ++seq);
       }
-      const uint32_t off = (uint32_t)(at - seq_begin), each = sp.steps + kSwitch;
+      const uint32_t off = (uint32_t)(at - seq_begin), each = sp.steps + C::change;
       unit = (int)(off / each);
       step0 = (int)(off - unit * each);
       if (step0 < sp.steps || at >= we) break;
@@ -752,9 +755,9 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
       // the blocks of the segment: cuts inside it, by the same rule as above
       int lo = x / per + 1, hi = (y_end - 1) / per;
 #pragma unroll 1
-      while (snapped(lo * per, x, y_end, near) == x) ++lo;
+      while (snapped<C::change>(lo * per, x, y_end, near) == x) ++lo;
 #pragma unroll 1
-      while (snapped(hi * per, x, y_end, near) == y_end) --hi;
+      while (snapped<C::change>(hi * per, x, y_end, near) == y_end) --hi;
       first = lo - 1;
       last = hi;
       at_seq = cut.seq;

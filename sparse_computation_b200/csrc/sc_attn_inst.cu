@@ -14,7 +14,7 @@ template <int MODE, int DP, bool FULL>
 Variant variant(int q_rows, int smem_limit) {
   using C = Cfg<MODE, DP>;
   const int per_warp = C::warp_bytes(q_rows);
-  Variant v{attend_kernel<MODE, DP, FULL>, 0, 0, C::keys, C::piece};
+  Variant v{attend_kernel<MODE, DP, FULL>, 0, 0, C::keys, C::piece, C::change};
   cudaFuncAttributes attr;
   cuda_check(cudaFuncGetAttributes(&attr, v.kernel), "kernel attributes");
   v.warps = std::min(C::max_warps, (smem_limit - (int)attr.sharedSizeBytes) / per_warp);
