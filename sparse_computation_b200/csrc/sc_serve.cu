@@ -14,13 +14,29 @@ constexpr int64_t kMaxHeadDim = 256;  // the widest tile of the attention kernel
 
 // --------------------------------------------------------------- append ----
 
+// n / by for n below 2^31, as umulhi(n, mul) >> shift (mul 0: by is 1).
+struct Divider {
+  uint32_t by = 1, mul = 0, shift = 0;
+  Divider() = default;
+  explicit Divider(int64_t d) : by((uint32_t)d) {
+    for (int bits = 1; d > 1; ++bits)
+      if (((int64_t)1 << bits) >= d) {
+        mul = (uint32_t)((((uint64_t)1 << (31 + bits)) + d - 1) / d);
+        shift = bits - 1;
+        return;
+      }
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return mul ? __umulhi(n, mul) >> shift : n; }
+};
+
 struct AppendParams {
   sc_kv_append_args a;
   sc_kv_pool pool;
   int *status;
   uint32_t page_mul, page_shift;    // divider by the page size
   uint32_t pairs_mul, pairs_shift;  // divider by the pairs of a head
-  int tile_bits, parts;
+  int tile_bits, parts, eights, rope4;
+  Divider plain, turned;            // eights of a head; without the partners' in the half style
 };
 
 // The cache place of token t: page and slot, or page -1 when it is skipped.
@@ -124,21 +140,6 @@ struct Eight {
   }
 };
 
-// n / by for n below 2^31, as umulhi(n, mul) >> shift (mul 0: by is 1).
-struct Divider {
-  uint32_t by = 1, mul = 0, shift = 0;
-  Divider() = default;
-  explicit Divider(int64_t d) : by((uint32_t)d) {
-    for (int bits = 1; d > 1; ++bits)
-      if (((int64_t)1 << bits) >= d) {
-        mul = (uint32_t)((((uint64_t)1 << (31 + bits)) + d - 1) / d);
-        shift = bits - 1;
-        return;
-      }
-  }
-  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return mul ? __umulhi(n, mul) >> shift : n; }
-};
-
 // Token-major activations (the heads of a token contiguous): a warp takes a
 // token, or 1/p.parts of it, so that position, page and rotation row are its
 // own scalars.  It walks the heads of v, k and q in jobs of eight dims (with
@@ -157,6 +158,38 @@ struct Turn {  // the rotation of a token
   int rotary;  // 0: none
   bool four;   // rows can be read in fours
 };
+
+// Turns dims d .. d + 7 (x), in the half style with their partners (z).
+__device__ __forceinline__ void turn8(float (&x)[8], float (&z)[8], int d, int half, const Turn &turn) {
+  const float *cp = turn.cos + (half ? d : d / 2), *sp = turn.sin + (half ? d : d / 2);
+  float c[8], s[8];
+#pragma unroll
+  for (int e = 0; e < 8; e += 4)
+    if (e == 0 || half) {
+      if (turn.four) {
+        *reinterpret_cast<float4 *>(c + e) = *reinterpret_cast<const float4 *>(cp + e);
+        *reinterpret_cast<float4 *>(s + e) = *reinterpret_cast<const float4 *>(sp + e);
+      } else {
+#pragma unroll
+        for (int f = e; f < e + 4; ++f) c[f] = cp[f], s[f] = sp[f];
+      }
+    }
+  if (half) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = x[e] * c[e] - z[e] * s[e];
+      z[e] = z[e] * c[e] + x[e] * s[e];
+      x[e] = v;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float v = x[e] * c[e / 2] - x[e + 1] * s[e / 2];
+      x[e + 1] = x[e + 1] * c[e / 2] + x[e] * s[e / 2];
+      x[e] = v;
+    }
+  }
+}
 
 // BATCH jobs of one lane, `step` apart.
 template <class T, int BATCH>
@@ -201,36 +234,7 @@ struct HeadJobs {
       float x[8], z[8] = {};
       u[i].get(x);
       if (two) w[i].get(z);
-      if (d < turn.rotary) {
-        const float *cp = turn.cos + (r.half ? d : d / 2), *sp = turn.sin + (r.half ? d : d / 2);
-        float c[8], s[8];
-#pragma unroll
-        for (int e = 0; e < 8; e += 4)
-          if (e == 0 || r.half) {
-            if (turn.four) {
-              *reinterpret_cast<float4 *>(c + e) = *reinterpret_cast<const float4 *>(cp + e);
-              *reinterpret_cast<float4 *>(s + e) = *reinterpret_cast<const float4 *>(sp + e);
-            } else {
-#pragma unroll
-              for (int f = e; f < e + 4; ++f) c[f] = cp[f], s[f] = sp[f];
-            }
-          }
-        if (r.half) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float v = x[e] * c[e] - z[e] * s[e];
-            z[e] = z[e] * c[e] + x[e] * s[e];
-            x[e] = v;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float v = x[e] * c[e / 2] - x[e + 1] * s[e / 2];
-            x[e + 1] = x[e + 1] * c[e / 2] + x[e] * s[e / 2];
-            x[e] = v;
-          }
-        }
-      }
+      if (d < turn.rotary) turn8(x, z, d, r.half, turn);
       if (zero)
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = z[e] = 0.f;
@@ -289,17 +293,20 @@ __global__ void __launch_bounds__(128, 4) append_rows_kernel(const __grid_consta
 
 // Feature-major activations, as a product leaves them (tokens contiguous): a
 // block takes one head of 2^p.tile_bits tokens, reads it along the tokens,
-// turns it in shared memory and writes it along the dims, two to a thread.
-// Bound by the chain of latencies (position, page entry, rotation row, store)
-// at decoding sizes: 128 tokens of 32 + 2 x 8 heads of 128, fp32 into bf16,
-// 6.9 us against 0.9 for their bytes; 4 tokens of 3 x 8 heads of 64 2.6 us.
+// turns it in shared memory and writes it along the dims, two to a thread, or
+// eight for prompts.  Bound by the chain of latencies (position, page entry,
+// rotation row, store) at decoding sizes: 128 tokens of 32 + 2 x 8 heads of 128,
+// fp32 into bf16, 4.3 us against 0.9 for their bytes; 4 tokens of 3 x 8 heads
+// of 64 2.1 us.
 template <class T, class C>
 __global__ void __launch_bounds__(256) append_columns_kernel(const __grid_constant__ AppendParams p) {
   const sc_kv_append_args &a = p.a;
-  __shared__ float tile[kMaxHeadDim * 33];
+  __shared__ float tile[kMaxHeadDim * 33 + kMaxHeadDim / 8];
   __shared__ int s_pos[32], s_slot[32], s_page[32];
   const int hk = (int)p.pool.kv_heads, hq = a.q.ptr ? (int)a.q_heads : 0, D = (int)p.pool.head_dim;
-  const int TT = 1 << p.tile_bits, width = TT + 1;
+  const int TT = 1 << p.tile_bits;
+  // a word more for each dim and each eight: neither the tokens of a dim nor every eighth dim of a token share a bank
+  auto place = [&](int d, int t) { return d * (TT + 1) + d / 8 + t; };
   const int64_t t0 = (int64_t)blockIdx.y << p.tile_bits;
   const int here = (int)min((int64_t)TT, a.tokens - t0);
   int head = blockIdx.x;
@@ -308,7 +315,7 @@ __global__ void __launch_bounds__(256) append_columns_kernel(const __grid_consta
   if (!is_q) head -= is_v ? hq + hk : hq;
   const T *x = static_cast<const T *>(src.ptr) + t0 + head * src.stride[1];
   // the first loads are on their way while the places, two dependent loads, are worked out
-  constexpr int B = 16;
+  constexpr int B = 4;
   auto load = [&](int i0, T (&v)[B]) {
 #pragma unroll
     for (int k = 0; k < B; ++k) {
@@ -320,7 +327,7 @@ __global__ void __launch_bounds__(256) append_columns_kernel(const __grid_consta
 #pragma unroll
     for (int k = 0; k < B; ++k) {
       const int i = i0 + 256 * k, d = i >> p.tile_bits, t = i & (TT - 1);
-      if (d < D && t < here) tile[d * width + t] = to_f32(v[k]);
+      if (d < D && t < here) tile[place(d, t)] = to_f32(v[k]);
     }
   };
   T v[B];
@@ -339,11 +346,45 @@ __global__ void __launch_bounds__(256) append_columns_kernel(const __grid_consta
   __syncthreads();
   const int rotary = a.cos && !is_v ? (int)a.rotary : 0, half = rotary / 2, pairs = D / 2;
   const bool halves = !a.interleaved;
+  if (p.eights) {
+    const int h = halves ? half : 0;
+    const Divider &by = h ? p.turned : p.plain;  // eights of a head, partners' apart
+    for (int i = threadIdx.x; i < (int)by.by * here; i += 256) {
+      const int t = (int)by(i), e = i - t * (int)by.by, d = e * 8 < h ? e * 8 : e * 8 + h;
+      const int page = s_page[t], pos = s_pos[t];
+      if (page < 0 && !is_q) continue;
+      const bool two = d < h;
+      float u[8], w[8] = {};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        u[k] = page < 0 ? 0.f : tile[place(d + k, t)];
+        if (two && page >= 0) w[k] = tile[place(d + h + k, t)];
+      }
+      if (d < rotary && page >= 0)
+        turn8(u, w, d, h, Turn{a.cos + pos * a.rope_stride, a.sin + pos * a.rope_stride, rotary, p.rope4 != 0});
+      auto put = [&](auto *y) {
+        Eight<std::remove_reference_t<decltype(*y)>> o;
+        o.set(u);
+        o.store(y);
+        if (two) {
+          o.set(w);
+          o.store(y + h);
+        }
+      };
+      if (is_q) {
+        put(static_cast<T *>(a.q_out.ptr) + (t0 + t) * a.q_out.stride[0] + head * a.q_out.stride[1] + d);
+      } else {
+        const int64_t *st = is_v ? p.pool.v_stride : p.pool.k_stride;
+        put(static_cast<C *>(is_v ? p.pool.v : p.pool.k) + page * st[0] + head * st[1] + s_slot[t] * st[2] + d);
+      }
+    }
+    return;
+  }
   for (int i = threadIdx.x; i < pairs * here; i += 256) {
     const int t = p.pairs_mul ? (int)(__umulhi(i, p.pairs_mul) >> p.pairs_shift) : i, d = 2 * (i - t * pairs);
     const int page = s_page[t], pos = s_pos[t];
     if (page < 0 && !is_q) continue;
-    float u = tile[d * width + t], w = tile[(d + 1) * width + t];
+    float u = tile[place(d, t)], w = tile[place(d + 1, t)];
     if (page < 0) {
       u = w = 0.f;
     } else if (d < rotary) {
@@ -352,8 +393,8 @@ __global__ void __launch_bounds__(256) append_columns_kernel(const __grid_consta
         const bool upper = d >= half;
         const int i0 = upper ? d - half : d, other = upper ? d - half : d + half;
         const float sign = upper ? 1.f : -1.f;
-        u = u * c[i0] + sign * (tile[other * width + t] * s[i0]);
-        w = w * c[i0 + 1] + sign * (tile[(other + 1) * width + t] * s[i0 + 1]);
+        u = u * c[i0] + sign * (tile[place(other, t)] * s[i0]);
+        w = w * c[i0 + 1] + sign * (tile[place(other + 1, t)] * s[i0 + 1]);
       } else {
         const float ci = c[d / 2], si = s[d / 2], ru = u * ci - w * si;
         w = w * ci + u * si;
@@ -462,7 +503,7 @@ int sc_kv_append(sc_kv_cache *c, const sc_kv_append_args *a, void *stream) {
     require(a->rotary > 0 && a->rotary % 2 == 0 && a->rotary <= c->pool.head_dim && a->rope_rows > 0, SC_ERR_ARG,
             "rotary must be even and at most head_dim");
   const Divider by_page(c->pool.page_size);
-  AppendParams p{*a, c->pool, static_cast<int *>(c->status.p), by_page.mul, by_page.shift, 0, 0, 0, 0};
+  AppendParams p{*a, c->pool, static_cast<int *>(c->status.p), by_page.mul, by_page.shift, 0, 0, 0, 0, 0, 0, Divider(), Divider()};
   DeviceGuard dg(c->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool q = a->q.ptr != nullptr, rotates = a->cos != nullptr, halves = rotates && !a->interleaved;
@@ -477,6 +518,13 @@ int sc_kv_append(sc_kv_cache *c, const sc_kv_append_args *a, void *stream) {
                             along_dims(a->q, a->tokens, a->type, 8) && along_dims(a->q_out, a->tokens, a->type, 8)));
   const bool columns = half % 2 == 0 && (!q || (a->q.stride[0] == 1 && along_dims(a->q_out, a->tokens, a->type, 2))) &&
                        a->k.stride[0] == 1 && a->v.stride[0] == 1 && heads <= 65535;
+  const int rope4 = rotates && a->rope_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a->cos) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(a->sin) % 16 == 0;
+  p.rope4 = rope4;
+  p.plain = Divider(std::max<int64_t>(1, D / 8));
+  p.turned = Divider(std::max<int64_t>(1, (D - (halves ? half : 0)) / 8));
+  // results in eights, unless the rotation splits one or q_out is not laid out for it
+  p.eights = D % 8 == 0 && half % 8 == 0 && (!q || along_dims(a->q_out, a->tokens, a->type, 8));
   const int64_t n = a->tokens * heads * (D / 2);
   require((n + 255) / 256 <= INT32_MAX, SC_ERR_UNSUPPORTED, "too many rows in one call");
   with_types(a->type, c->pool.type, [&](auto t, auto e) {
@@ -485,8 +533,6 @@ int sc_kv_append(sc_kv_cache *c, const sc_kv_append_args *a, void *stream) {
     if (rows) {
       const int h = halves ? (int)half : 0;
       const RowJobs turned{Divider((D - h) / 8), h}, plain{Divider(D / 8), 0};
-      const int rope4 = rotates && a->rope_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a->cos) % 16 == 0 &&
-                        reinterpret_cast<uintptr_t>(a->sin) % 16 == 0;
       // one warp a token when that fills the SMs (16 warps each), else up to 8 warps
       p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(8, 148 * 16 / a->tokens));
       append_rows_kernel<T, C><<<dim3((unsigned)((a->tokens + 3) / 4), p.parts), 128, 0, st>>>(p, turned, plain, rope4);
@@ -496,6 +542,8 @@ int sc_kv_append(sc_kv_cache *c, const sc_kv_append_args *a, void *stream) {
       p.tile_bits = 5;
       while (p.tile_bits > fewest && heads * (a->tokens >> p.tile_bits) < 4 * 148) --p.tile_bits;
       while (p.tile_bits > 2 && a->tokens <= 1 << (p.tile_bits - 1)) --p.tile_bits;
+      // eights have fewer instructions, pairs more threads: 2000 tokens 21.3 us against 23.8, 128 tokens 5.2 against 4.3
+      if (p.tile_bits < 5) p.eights = 0;
       const Divider pairs(D / 2);
       p.pairs_mul = pairs.mul, p.pairs_shift = pairs.shift;
       append_columns_kernel<T, C>
