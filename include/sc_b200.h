@@ -367,6 +367,11 @@ typedef struct sc_attn sc_attn; /* decode-attention plan: head layout and worksp
  * must not overlap on the GPU. */
 int sc_attn_create(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, double scale, int64_t window,
                    sc_attn **out);
+/* The same in the caller's workspace: 256-byte aligned device memory of the
+ * size that sc_attn_workspace gives, which outlives the plan. */
+int sc_attn_workspace(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, int64_t *bytes);
+int sc_attn_create_in(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, double scale, int64_t window,
+                      void *workspace, int64_t workspace_bytes, sc_attn **out);
 void sc_attn_free(sc_attn *p);
 
 typedef struct sc_attn_args {
@@ -395,6 +400,14 @@ int sc_adapters_create(int32_t device, int64_t in_features, int64_t out_features
                        const int64_t *ranks, int64_t type, const void *const *down, const int64_t *down_ld,
                        const void *const *up, const int64_t *up_ld, const float *scales, void *stream,
                        sc_adapters **out);
+/* The same in the caller's memory: 256-byte aligned device memory of the size
+ * that sc_adapters_size gives, which outlives the set. */
+int sc_adapters_size(int64_t in_features, int64_t out_features, int64_t count, const int64_t *ranks, int64_t type,
+                     int64_t *bytes);
+int sc_adapters_create_in(int32_t device, int64_t in_features, int64_t out_features, int64_t count,
+                          const int64_t *ranks, int64_t type, const void *const *down, const int64_t *down_ld,
+                          const void *const *up, const int64_t *up_ld, const float *scales, void *stream,
+                          void *memory, int64_t memory_bytes, sc_adapters **out);
 void sc_adapters_free(sc_adapters *s);
 /* Scratch bytes that a call with this many tokens needs. */
 int sc_adapters_workspace(const sc_adapters *s, int64_t tokens, int64_t *bytes);

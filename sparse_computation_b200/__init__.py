@@ -67,8 +67,8 @@ EXPORTED_SYMBOLS = (
     "sc_spmm_dense_noalloc", "sc_noalloc_status", "sc_plan_status", "sc_batch_status",
     "sc_graph_capture_plan", "sc_graph_capture_batch", "sc_graph_launch", "sc_graph_free",
     "sc_kv_cache_create", "sc_kv_cache_free", "sc_kv_cache_status", "sc_kv_append",
-    "sc_attn_create", "sc_attn_free", "sc_attn_decode", "sc_attn_status",
-    "sc_adapters_create", "sc_adapters_free", "sc_adapters_workspace", "sc_adapters_apply", "sc_adapters_status",
+    "sc_attn_create", "sc_attn_create_in", "sc_attn_workspace", "sc_attn_free", "sc_attn_decode", "sc_attn_status",
+    "sc_adapters_create", "sc_adapters_create_in", "sc_adapters_size", "sc_adapters_free", "sc_adapters_workspace", "sc_adapters_apply", "sc_adapters_status",
 )
 
 
@@ -156,10 +156,14 @@ def lib() -> ctypes.CDLL:
         "sc_kv_cache_status": ([vp, P(i32)], ctypes.c_int),
         "sc_kv_append": ([vp, vp, vp], ctypes.c_int),
         "sc_attn_create": ([vp, i64, i64, ctypes.c_double, i64, P(vp)], ctypes.c_int),
+        "sc_attn_create_in": ([vp, i64, i64, ctypes.c_double, i64, vp, i64, P(vp)], ctypes.c_int),
+        "sc_attn_workspace": ([vp, i64, i64, P(i64)], ctypes.c_int),
         "sc_attn_free": ([vp], None),
         "sc_attn_decode": ([vp, vp, vp], ctypes.c_int),
         "sc_attn_status": ([vp, P(i32)], ctypes.c_int),
         "sc_adapters_create": ([i32, i64, i64, i64, vp, i64, vp, vp, vp, vp, vp, vp, P(vp)], ctypes.c_int),
+        "sc_adapters_create_in": ([i32, i64, i64, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, P(vp)], ctypes.c_int),
+        "sc_adapters_size": ([i64, i64, i64, vp, i64, P(i64)], ctypes.c_int),
         "sc_adapters_free": ([vp], None),
         "sc_adapters_workspace": ([vp, i64, P(i64)], ctypes.c_int),
         "sc_adapters_apply": ([vp, vp, vp], ctypes.c_int),

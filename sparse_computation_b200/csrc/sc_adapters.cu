@@ -35,11 +35,20 @@ struct SetView {
   int *status;
 };
 
+// Copies matrix blockIdx.y of `list` into rows of dst_row elements, padded with zeros.
+struct PackItem {
+  const void *src;
+  int64_t row_stride, col_stride, cols, dst_row, dst;  // dst: first element
+  int rows;
+};
 template <class W>
-__global__ void pack_rows(const W *src, int64_t row_stride, int64_t col_stride, int64_t rows, int64_t cols, W *dst,
-                          int64_t dst_row) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, r = i / dst_row, c = i % dst_row;
-  if (r < rows) dst[i] = c < cols ? src[r * row_stride + c * col_stride] : W(0);
+__global__ void __launch_bounds__(256) pack_rows(const PackItem *list, W *dst) {
+  const PackItem p = list[blockIdx.y];
+  const W *src = static_cast<const W *>(p.src);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.rows * p.dst_row; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / p.dst_row, c = i % p.dst_row;
+    dst[p.dst + i] = c < p.cols ? src[r * p.row_stride + c * p.col_stride] : W(0);
+  }
 }
 
 // ------------------------------------------------------ a few tokens ----
@@ -787,70 +796,129 @@ struct sc_adapters {
   int64_t type = 0;
   SetView view{};
   int64_t mean_bytes = 0;  // of an adapter's weights
-  DeviceBlock mem;
+  DeviceBlock mem;  // its own memory, if any
 };
 
+namespace {
+
+// Where a set's parts lie in its memory.
+struct SetLayout {
+  std::vector<int32_t> first;
+  int64_t total = 0, most = 0, in_row = 0, out_row = 0, filled = 0;  // filled: adapters with ranks
+  size_t e = 0, up = 0, firsts = 0, scales = 0, status = 0, list = 0, bytes = 0;
+};
+
+SetLayout lay_out(int64_t in_features, int64_t out_features, int64_t count, const int64_t *ranks, int64_t type) {
+  require(count > 0 && count < (1 << 24), SC_ERR_ARG, "a set has 1 to 2^24 adapters");
+  require(in_features > 0 && out_features > 0 && in_features < (1 << 24) && out_features < (1 << 24), SC_ERR_ARG,
+          "features must be 1 to 2^24");
+  require(type_ok(type), SC_ERR_ARG, "unknown element type");
+  SetLayout l;
+  l.first.assign(count + 1, 0);
+  for (int64_t i = 0; i < count; ++i) {
+    require(ranks[i] >= 0 && ranks[i] <= kMaxRank, SC_ERR_UNSUPPORTED, "ranks must be 0 to 256");
+    l.total += ranks[i];
+    l.most = std::max(l.most, ranks[i]);
+    l.filled += ranks[i] > 0;
+    require(l.total < INT32_MAX, SC_ERR_UNSUPPORTED, "too many rank rows in one set");
+    l.first[i + 1] = (int32_t)l.total;
+  }
+  l.e = (size_t)type_bytes(type);
+  l.in_row = (in_features + kPad - 1) / kPad * kPad;
+  l.out_row = (out_features + kPad - 1) / kPad * kPad;
+  l.up = align256(l.total * l.in_row * l.e + 16);
+  l.firsts = l.up + align256(l.total * l.out_row * l.e + 16);
+  l.scales = l.firsts + align256((count + 1) * 4);
+  l.status = l.scales + align256(count * 4);
+  l.list = l.status + 256;
+  l.bytes = l.list + align256(2 * l.filled * sizeof(PackItem));
+  return l;
+}
+
+// memory null: the set allocates it.
+sc_adapters *make_set(int32_t device, int64_t in_features, int64_t out_features, int64_t count, const int64_t *ranks,
+                      int64_t type, const void *const *down, const int64_t *down_ld, const void *const *up,
+                      const int64_t *up_ld, const float *scales, cudaStream_t st, void *memory, int64_t bytes) {
+  require(ranks && down && down_ld && up && up_ld && scales, SC_ERR_ARG, "null argument");
+  require(device >= 0 && device < 64, SC_ERR_ARG, "bad device");
+  const SetLayout l = lay_out(in_features, out_features, count, ranks, type);
+  for (int64_t i = 0; i < count; ++i)
+    require(ranks[i] == 0 || (down[i] && up[i] && down_ld[i] >= in_features && up_ld[i] >= ranks[i]), SC_ERR_ARG,
+            "null adapter weights or row stride too small");
+  require(!memory || (bytes >= (int64_t)l.bytes && reinterpret_cast<uintptr_t>(memory) % 256 == 0), SC_ERR_ARG,
+          "memory too small or not 256-byte aligned");
+  std::unique_ptr<sc_adapters> s(new sc_adapters);
+  s->device = device;
+  s->type = type;
+  DeviceGuard dg(device);
+  if (!memory) {
+    s->mem.alloc(device, l.bytes, "allocate adapters");
+    memory = s->mem.p;
+  }
+  uint8_t *p = static_cast<uint8_t *>(memory);
+  cuda_check(cudaMemcpyAsync(p + l.firsts, l.first.data(), (count + 1) * 4, cudaMemcpyHostToDevice, st), "upload adapters");
+  cuda_check(cudaMemcpyAsync(p + l.scales, scales, count * 4, cudaMemcpyHostToDevice, st), "upload adapters");
+  cuda_check(cudaMemsetAsync(p + l.status, 0, 256, st), "clear status word");
+  std::vector<PackItem> list;
+  list.reserve(2 * l.filled);
+  for (int64_t i = 0; i < count; ++i) {
+    if (!ranks[i]) continue;
+    list.push_back({down[i], down_ld[i], 1, in_features, l.in_row, l.first[i] * l.in_row, (int)ranks[i]});
+    list.push_back({up[i], 1, up_ld[i], out_features, l.out_row, (int64_t)(l.up / l.e) + l.first[i] * l.out_row, (int)ranks[i]});
+  }
+  if (!list.empty())
+    cuda_check(cudaMemcpyAsync(p + l.list, list.data(), list.size() * sizeof(PackItem), cudaMemcpyHostToDevice, st),
+               "upload packing list");
+  const unsigned across = (unsigned)std::max<int64_t>(1, std::min<int64_t>(64, l.most * std::max(l.in_row, l.out_row) / 1024));
+  for (size_t at = 0; at < list.size(); at += 65535) {
+    const dim3 grid(across, (unsigned)std::min<size_t>(65535, list.size() - at));
+    const PackItem *items = reinterpret_cast<const PackItem *>(p + l.list) + at;
+    if (l.e == 4)
+      pack_rows<<<grid, 256, 0, st>>>(items, reinterpret_cast<uint32_t *>(p));
+    else
+      pack_rows<<<grid, 256, 0, st>>>(items, reinterpret_cast<uint16_t *>(p));
+  }
+  cuda_check(cudaGetLastError(), "launch adapter packing");
+  cuda_check(cudaStreamSynchronize(st), "stream synchronize");
+  s->view = SetView{p,           p + l.up,     reinterpret_cast<int32_t *>(p + l.firsts), reinterpret_cast<float *>(p + l.scales),
+                    in_features, out_features, l.in_row, l.out_row, (int)count, (int)l.most, reinterpret_cast<int *>(p + l.status)};
+  s->mean_bytes = (int64_t)(l.firsts / count);
+  return s.release();
+}
+
+}  // namespace
+
 extern "C" {
+
+int sc_adapters_size(int64_t in_features, int64_t out_features, int64_t count, const int64_t *ranks, int64_t type,
+                     int64_t *bytes) {
+  SC_SERVE_BEGIN
+  require(ranks && bytes, SC_ERR_ARG, "null argument");
+  *bytes = (int64_t)lay_out(in_features, out_features, count, ranks, type).bytes;
+  SC_SERVE_END
+}
 
 int sc_adapters_create(int32_t device, int64_t in_features, int64_t out_features, int64_t count,
                        const int64_t *ranks, int64_t type, const void *const *down, const int64_t *down_ld,
                        const void *const *up, const int64_t *up_ld, const float *scales, void *stream,
                        sc_adapters **out) {
   SC_SERVE_BEGIN
-  require(out && ranks && down && down_ld && up && up_ld && scales, SC_ERR_ARG, "null argument");
+  require(out, SC_ERR_ARG, "null argument");
   *out = nullptr;
-  require(device >= 0 && device < 64, SC_ERR_ARG, "bad device");
-  require(count > 0 && count < (1 << 24), SC_ERR_ARG, "a set has 1 to 2^24 adapters");
-  require(in_features > 0 && out_features > 0 && in_features < (1 << 24) && out_features < (1 << 24), SC_ERR_ARG,
-          "features must be 1 to 2^24");
-  require(type_ok(type), SC_ERR_ARG, "unknown element type");
-  std::vector<int32_t> first(count + 1, 0);
-  int64_t total = 0, most = 0;
-  for (int64_t i = 0; i < count; ++i) {
-    require(ranks[i] >= 0 && ranks[i] <= kMaxRank, SC_ERR_UNSUPPORTED, "ranks must be 0 to 256");
-    require(ranks[i] == 0 || (down[i] && up[i] && down_ld[i] >= in_features && up_ld[i] >= ranks[i]), SC_ERR_ARG,
-            "null adapter weights or row stride too small");
-    total += ranks[i];
-    most = std::max(most, ranks[i]);
-    require(total < INT32_MAX, SC_ERR_UNSUPPORTED, "too many rank rows in one set");
-    first[i + 1] = (int32_t)total;
-  }
-  const size_t e = (size_t)type_bytes(type);
-  const int64_t in_row = (in_features + kPad - 1) / kPad * kPad, out_row = (out_features + kPad - 1) / kPad * kPad;
-  const size_t b_down = align256(total * in_row * e + 16), b_up = align256(total * out_row * e + 16);
-  const size_t b_first = align256((count + 1) * 4), b_scale = align256(count * 4);
-  std::unique_ptr<sc_adapters> s(new sc_adapters);
-  s->device = device;
-  s->type = type;
-  DeviceGuard dg(device);
-  s->mem.alloc(device, b_down + b_up + b_first + b_scale + 256, "allocate adapters");
-  uint8_t *p = static_cast<uint8_t *>(s->mem.p);
-  uint8_t *d_down = p, *d_up = d_down + b_down, *d_first = d_up + b_up, *d_scale = d_first + b_first,
-          *d_status = d_scale + b_scale;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cuda_check(cudaMemcpyAsync(d_first, first.data(), (count + 1) * 4, cudaMemcpyHostToDevice, st), "upload adapters");
-  cuda_check(cudaMemcpyAsync(d_scale, scales, count * 4, cudaMemcpyHostToDevice, st), "upload adapters");
-  cuda_check(cudaMemsetAsync(d_status, 0, 256, st), "clear status word");
-  auto pack = [&](const void *src, int64_t rs, int64_t cs, int64_t rows, int64_t cols, uint8_t *dst, int64_t dst_row) {
-    const unsigned blocks = (unsigned)((rows * dst_row + 255) / 256);
-    if (e == 4)
-      pack_rows<<<blocks, 256, 0, st>>>(static_cast<const uint32_t *>(src), rs, cs, rows, cols,
-                                        reinterpret_cast<uint32_t *>(dst), dst_row);
-    else
-      pack_rows<<<blocks, 256, 0, st>>>(static_cast<const uint16_t *>(src), rs, cs, rows, cols,
-                                        reinterpret_cast<uint16_t *>(dst), dst_row);
-  };
-  for (int64_t i = 0; i < count; ++i) {
-    if (!ranks[i]) continue;
-    pack(down[i], down_ld[i], 1, ranks[i], in_features, d_down + (size_t)first[i] * in_row * e, in_row);
-    pack(up[i], 1, up_ld[i], ranks[i], out_features, d_up + (size_t)first[i] * out_row * e, out_row);
-  }
-  cuda_check(cudaGetLastError(), "launch adapter packing");
-  cuda_check(cudaStreamSynchronize(st), "stream synchronize");
-  s->view = SetView{d_down,          d_up,        reinterpret_cast<int32_t *>(d_first), reinterpret_cast<float *>(d_scale),
-                    in_features,     out_features, in_row, out_row, (int)count, (int)most, reinterpret_cast<int *>(d_status)};
-  s->mean_bytes = (int64_t)((b_down + b_up) / count);
-  *out = s.release();
+  *out = make_set(device, in_features, out_features, count, ranks, type, down, down_ld, up, up_ld, scales,
+                  static_cast<cudaStream_t>(stream), nullptr, 0);
+  SC_SERVE_END
+}
+
+int sc_adapters_create_in(int32_t device, int64_t in_features, int64_t out_features, int64_t count,
+                          const int64_t *ranks, int64_t type, const void *const *down, const int64_t *down_ld,
+                          const void *const *up, const int64_t *up_ld, const float *scales, void *stream,
+                          void *memory, int64_t memory_bytes, sc_adapters **out) {
+  SC_SERVE_BEGIN
+  require(out && memory, SC_ERR_ARG, "null argument");
+  *out = nullptr;
+  *out = make_set(device, in_features, out_features, count, ranks, type, down, down_ld, up, up_ld, scales,
+                  static_cast<cudaStream_t>(stream), memory, memory_bytes);
   SC_SERVE_END
 }
 

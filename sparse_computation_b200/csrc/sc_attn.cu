@@ -16,18 +16,20 @@ struct sc_attn {
   int qtiles = 0, q_rows = 0, sms = 0;
   uint32_t page_mul = 0, page_shift = 0;
   Variant same, other;  // q of the cache's type; q of another type
-  DeviceBlock mem;      // status | 1 KB of zeros | arrivals | pieces | records
+  DeviceBlock mem;      // its own workspace, if any: status | 1 KB of zeros | arrivals | pieces | records
   int *status = nullptr, *arrivals = nullptr;
   float *heads = nullptr, *records = nullptr;
 };
 
-extern "C" {
+namespace {
 
-int sc_attn_create(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, double scale, int64_t window,
-                   sc_attn **out) {
-  SC_SERVE_BEGIN
-  require(cache && out, SC_ERR_ARG, "null argument");
-  *out = nullptr;
+// A plan without its workspace, and the layout of that in 4-byte words.
+struct Layout {
+  size_t words, heads, total;  // status, zeros and arrivals; pieces; all
+};
+
+std::unique_ptr<sc_attn> set_up(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, double scale, int64_t window,
+                                Layout &layout) {
   const sc_kv_pool &pool = cache->pool;
   require(q_heads > 0 && q_heads % pool.kv_heads == 0 && q_heads <= 65535, SC_ERR_ARG,
           "q_heads must be a positive multiple of kv_heads");
@@ -72,15 +74,60 @@ int sc_attn_create(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, 
     p->other = p->q_rows <= 4 ? variant_for<kBF16Wide4>(pool.head_dim, p->q_rows, limit)
                               : variant_for<kBF16Wide>(pool.head_dim, p->q_rows, limit);
   }
-  const size_t words = 64 + 256 + ((size_t)segments + 63) / 64 * 64, piece = (size_t)p->same.piece;
-  const size_t heads = (size_t)p->sms * std::max(p->same.warps, p->other.warps) * piece;
-  p->mem.alloc(p->device, (words + heads + (size_t)p->sms * 2 * piece) * 4, "allocate attention workspace");
-  cuda_check(cudaMemset(p->mem.p, 0, words * 4), "clear attention workspace");
-  cuda_check(cudaDeviceSynchronize(), "device synchronize");
-  p->status = static_cast<int *>(p->mem.p);
-  p->arrivals = p->status + 64 + 256;
-  p->heads = reinterpret_cast<float *>(p->status + words);
-  p->records = p->heads + heads;
+  const size_t piece = (size_t)p->same.piece;
+  layout.words = 64 + 256 + ((size_t)segments + 63) / 64 * 64;
+  layout.heads = (size_t)p->sms * std::max(p->same.warps, p->other.warps) * piece;
+  layout.total = layout.words + layout.heads + (size_t)p->sms * 2 * piece;
+  return p;
+}
+
+void give_workspace(sc_attn &p, void *at, const Layout &layout) {
+  cuda_check(cudaMemset(at, 0, layout.words * 4), "clear attention workspace");
+  cuda_check(cudaStreamSynchronize(nullptr), "stream synchronize");
+  p.status = static_cast<int *>(at);
+  p.arrivals = p.status + 64 + 256;
+  p.heads = reinterpret_cast<float *>(p.status + layout.words);
+  p.records = p.heads + layout.heads;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sc_attn_workspace(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, int64_t *bytes) {
+  SC_SERVE_BEGIN
+  require(cache && bytes, SC_ERR_ARG, "null argument");
+  Layout layout;
+  set_up(cache, q_heads, max_seqs, 1.0, 0, layout);
+  *bytes = (int64_t)layout.total * 4;
+  SC_SERVE_END
+}
+
+int sc_attn_create(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, double scale, int64_t window,
+                   sc_attn **out) {
+  SC_SERVE_BEGIN
+  require(cache && out, SC_ERR_ARG, "null argument");
+  *out = nullptr;
+  Layout layout;
+  auto p = set_up(cache, q_heads, max_seqs, scale, window, layout);
+  DeviceGuard dg(p->device);
+  p->mem.alloc(p->device, layout.total * 4, "allocate attention workspace");
+  give_workspace(*p, p->mem.p, layout);
+  *out = p.release();
+  SC_SERVE_END
+}
+
+int sc_attn_create_in(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, double scale, int64_t window,
+                      void *workspace, int64_t workspace_bytes, sc_attn **out) {
+  SC_SERVE_BEGIN
+  require(cache && out && workspace, SC_ERR_ARG, "null argument");
+  *out = nullptr;
+  Layout layout;
+  auto p = set_up(cache, q_heads, max_seqs, scale, window, layout);
+  require(workspace_bytes >= (int64_t)layout.total * 4 && reinterpret_cast<uintptr_t>(workspace) % 256 == 0, SC_ERR_ARG,
+          "workspace too small or not 256-byte aligned");
+  DeviceGuard dg(p->device);
+  give_workspace(*p, workspace, layout);
   *out = p.release();
   SC_SERVE_END
 }

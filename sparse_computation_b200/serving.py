@@ -237,8 +237,13 @@ class DecodeAttention(_Handle):
             _fail("scale must be positive")
         self.cache, self.q_heads, self.max_seqs, self.window = cache, q_heads, max_seqs, window
         self.device = cache.device
-        h = ctypes.c_void_p()
-        _check(lib().sc_attn_create(cache._h, q_heads, max_seqs, scale or 0.0, window, ctypes.byref(h)))
+        h, size = ctypes.c_void_p(), ctypes.c_int64()
+        _check(lib().sc_attn_workspace(cache._h, q_heads, max_seqs, ctypes.byref(size)))
+        # from torch's allocator: a cudaMalloc and cudaFree for each plan took ten times as long as the rest
+        self._work = torch.empty(size.value + 256, dtype=torch.uint8, device=cache.k.device)
+        torch.cuda.current_stream(self.device).synchronize()  # whatever used that memory before is done
+        at = (self._work.data_ptr() + 255) // 256 * 256
+        _check(lib().sc_attn_create_in(cache._h, q_heads, max_seqs, scale or 0.0, window, at, size.value, ctypes.byref(h)))
         self._own(h)
 
     def attend(self, q, page_table, seq_lens, out=None, return_lse: bool = False, stream=None):
@@ -266,7 +271,7 @@ class DecodeAttention(_Handle):
         lse = q.new_empty((n, self.q_heads), dtype=torch.float32) if return_lse else None
         if n:
             s = _current(dev) if stream is None else _on(stream, dev, q, out, page_table, seq_lens, lse, self.cache.k,
-                                                         self.cache.v)
+                                                         self.cache.v, self._work)
             bad = self._call(self._h, _ATTEND.pack(n, kind, *qa, *oa, lse.data_ptr() if return_lse else 0, tab, cols,
                                                    tstride, lens), s)
             if bad:
@@ -305,12 +310,14 @@ class LowRankAdapters(_Handle):
         # a single row's stride means nothing: give the row length
         dl = [a.stride(0) if a.shape[0] > 1 else max(a.shape[1], 1) for a in down]
         ul = [b.stride(0) if b.shape[0] > 1 else max(b.shape[1], 1) for b in up]
-        h = ctypes.c_void_p()
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        _check(lib().sc_adapters_create(
-            self.device, self.in_features, self.out_features, n, i64(*ranks), _TYPES[dtype],
+        h, size, r = ctypes.c_void_p(), ctypes.c_int64(), i64(*ranks)
+        _check(lib().sc_adapters_size(self.in_features, self.out_features, n, r, _TYPES[dtype], ctypes.byref(size)))
+        self._memory = torch.empty(size.value + 256, dtype=torch.uint8, device=where)
+        at = (self._memory.data_ptr() + 255) // 256 * 256
+        _check(lib().sc_adapters_create_in(
+            self.device, self.in_features, self.out_features, n, r, _TYPES[dtype],
             vp(*[a.data_ptr() for a in down]), i64(*dl), vp(*[b.data_ptr() for b in up]), i64(*ul),
-            (ctypes.c_float * n)(*[float(x) for x in scales]), stream, ctypes.byref(h)))
+            (ctypes.c_float * n)(*[float(x) for x in scales]), _current(self.device), at, size.value, ctypes.byref(h)))
         self._own(h)
         self.ranks = ranks
         self._scratch = (-1, 0)
@@ -348,7 +355,7 @@ class LowRankAdapters(_Handle):
         if n:
             size = self._workspace(n)
             work = x.new_empty(size, dtype=torch.uint8) if size else None
-            s = _current(dev) if stream is None else _on(stream, dev, x, ids, base, out, work)
+            s = _current(dev) if stream is None else _on(stream, dev, x, ids, base, out, work, self._memory)
             bad = self._call(self._h, _ADAPT.pack(n, kind, *xa, *ba, *oa, idp, work.data_ptr() if size else 0, size), s)
             if bad:
                 _check(bad)
