@@ -736,8 +736,8 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
   }
 
   __syncthreads();
-  // ---- Round 0: the block's pieces, a warp per segment and row; the sums of segments that pass the run's ends become
-  // records.  Rounds 1 and 2: for the segments that pass its begin and its end, the last block to arrive adds their
+  // ---- Phase 0: the block's pieces, a warp per segment and row; the sums of segments that pass the run's ends become
+  // records.  Phases 1 and 2: for the segments that pass its begin and its end, the last block to arrive adds their
   // records up.
   const bool has = lane < 2 * W && s_seq[lane] >= 0;
   const uint32_t valid = __ballot_sync(~0u, has), earlier = valid & ((1u << lane) - 1);
@@ -746,12 +746,12 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
       __ballot_sync(~0u, has && (!earlier || s_seq[prev] != s_seq[lane] || s_unit[prev] != s_unit[lane]));
   constexpr int ND = (DP + 127) / 128;
 #pragma unroll 1
-  for (int round = 0; round < 3; ++round) {
+  for (int phase = 0; phase < 3; ++phase) {
     int tasks = __popc(lead_mask) * p.q_rows, first = 0, last = 0, at_seq = 0, at_unit = 0;
-    if (round) {
-      const Cut cut = s_cut[round - 1];
+    if (phase) {
+      const Cut cut = s_cut[phase - 1];
       const int x = cut.seg_begin, y_end = cut.seg_end;
-      if (cut.at <= x || cut.at >= y_end || (round == 2 && x < begin)) continue;
+      if (cut.at <= x || cut.at >= y_end || (phase == 2 && x < begin)) continue;
       // the blocks of the segment: cuts inside it, by the same rule as above
       int lo = x / per + 1, hi = (y_end - 1) / per;
 #pragma unroll 1
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
     for (int task = warp; task < tasks; task += W) {
       int r = task, record = 0;
       uint32_t members = 0;
-      if (!round) {
+      if (!phase) {
         r = task % p.q_rows;
         uint32_t leaders = lead_mask;
 #pragma unroll 1
@@ -802,7 +802,7 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
       for (int b = first; b <= last; b += 32) {
         const float *mine = nullptr;
         int here = 32;
-        if (round) {
+        if (phase) {
           here = min(32, last - b + 1);
           if (lane < here) mine = p.records + ((int64_t)(b + lane) * 2 + (b + lane == first)) * C::piece;
         } else if (members >> lane & 1) {

@@ -198,8 +198,10 @@ class PagedKVCache(_Handle):
             qa = _rows(q, "q", dev, qshape, dtype)
             if q_out is None:
                 q_out = q.new_empty(qshape)
-            oa = _rows(q_out, "q_out", dev, qshape, dtype)
-            _apart(q_out, "q_out")
+                oa = (q_out.data_ptr(), heads * self.head_dim, self.head_dim, 1)
+            else:
+                oa = _rows(q_out, "q_out", dev, qshape, dtype)
+                _apart(q_out, "q_out")
             if n and oa[0] == qa[0] and oa != qa:
                 _fail("q_out may only share q's memory with the same strides")
         elif q_out is not None:
@@ -262,8 +264,10 @@ class DecodeAttention(_Handle):
         qa = _rows(q, "q", dev, shape, dtype)
         if out is None:
             out = q.new_empty(shape)
-        oa = _rows(out, "out", dev, shape, dtype)
-        _apart(out, "out")
+            oa = (out.data_ptr(), self.q_heads * self.cache.head_dim, self.cache.head_dim, 1)
+        else:
+            oa = _rows(out, "out", dev, shape, dtype)
+            _apart(out, "out")
         tab, rows, cols, tstride = _table(page_table, dev)
         if rows < n:
             _fail(f"{n} sequences need a page table of as many rows, got {rows}")
@@ -345,8 +349,10 @@ class LowRankAdapters(_Handle):
         if out is None:
             # laid out as x is: feature-major, or token-major from a transposed x
             out = x.new_empty((n, self.out_features)).t() if xa[1] == 1 and n > 1 else x.new_empty(shape)
-        oa = _rows(out, "out", dev, shape, dtype)
-        _apart(out, "out")
+            oa = (out.data_ptr(), *out.stride())
+        else:
+            oa = _rows(out, "out", dev, shape, dtype)
+            _apart(out, "out")
         if n and oa[0] == ba[0] and oa != ba:
             _fail("out may only share base's memory with the same strides")
         if n and oa[0] == xa[0]:
