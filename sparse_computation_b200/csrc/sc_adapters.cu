@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewBlocks) few_kernel(const __gr
 // A block sorts the tokens by adapter first (group_kernel, 7 us for 2049
 // tokens); tokens without one are copied.  x and out bound it at best; at
 // present the latencies between the phases of a tile do, two blocks a SM:
-// 2049 fp32 tokens of 6 adapters, 2048 x 2048 in fp16, 55.9 us (one warp per
+// 2049 fp32 tokens of 6 adapters, 2048 x 2048 in fp16, 54.9 us (one warp per
 // token and rank row, then one thread per result: 387).
 constexpr int kMaxCluster = 8, kTile = 16, kChunk = 512, kThreads = 256, kWarps = kThreads / 32;
 constexpr int kXRow = kChunk + 4, kSpan = 64;  // floats of a token's chunk in shared memory; columns of a warp
@@ -378,10 +378,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   // this block's columns of x and rows of out
   const int k0 = (int)(s.in_row / blocks) * c, k1 = min((int)s.in, k0 + (int)(s.in_row / blocks));
   const int m0 = (int)(s.out_row / blocks) * c, m1 = min((int)s.out, m0 + (int)(s.out_row / blocks));
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if ((int)blockIdx.y >= *sorted.n) return;  // the whole cluster
   const Tile tile = sorted.tiles[blockIdx.y];
-  const int id = tile.adapter, n = tile.n;
+  const int n = tile.n;
   if (tid < n) s_tokens[tid] = sorted.tokens[tile.first + tid];
+  const int id = tile.adapter >= 0 && s.first[tile.adapter + 1] > s.first[tile.adapter] ? tile.adapter : -1;
   __syncthreads();
   if (id < 0) {
     if (a.out.ptr == a.base.ptr) return;
@@ -697,8 +699,9 @@ __global__ void __launch_bounds__(1024) group_kernel(const __grid_constant__ Set
   auto bin_of = [&](int i) {
     const int id = ids[i];
     if (id >= s.count) set_status(s.status, 10);
-    return id < 0 || id >= s.count || s.first[id + 1] == s.first[id] ? s.count : id;
+    return id < 0 || id >= s.count ? s.count : id;
   };
+  asm volatile("griddepcontrol.launch_dependents;");  // the tiles' blocks may take their places, and wait there
   for (int i = tid; i < bins; i += 1024) heads[i] = 0;
   if (tid == 0) s_tokens = s_tiles = 0;
   __syncthreads();
@@ -969,16 +972,18 @@ int sc_adapters_apply(sc_adapters *s, const sc_adapters_args *a, void *stream) {
       while (blocks > 2 && clusters * blocks > 4 * 148 && s->mean_bytes / blocks < 32 << 10) blocks /= 2;
     else
       while (blocks > 2 && clusters * blocks > 2 * 148) blocks /= 2;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = blocks;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = blocks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the tiles are launched while they are sorted
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(blocks, (unsigned)clusters);
     cfg.blockDim = dim3(few ? kFewThreads : kThreads);
     cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = few ? 1 : 2;
     if (few) {
       cuda_check(cudaLaunchKernelEx(&cfg, few_kernel<T, W>, s->view, *a), "launch adapters");
       return;
