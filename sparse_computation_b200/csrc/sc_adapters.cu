@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(256) pack_rows(const PackItem *list, W *dst) {
 // weights) and fp32 instructions; the tensor-core tiles below have twice the
 // fixed cost: 128 tokens of 100 adapters of 512 x 2048 in bf16 take 15.4 us
 // here, 28.6 there; 96 tokens of 40 adapters of 4096 x 4096 22.7 and 33.3.
-constexpr int kFewTokens = 256, kGroup = 4, kFewChunk = 512, kFewThreads = 256, kFewBlocks = 3;
+constexpr int kFewTokens = 256, kGroup = 4 /* a float4 of v */, kFewChunk = 512, kFewThreads = 256, kFewBlocks = 3;
 
 // Eight weights, as they lie.
 template <class W>
@@ -82,17 +82,20 @@ struct Eight {
   }
 };
 
-// 16-byte aligned: x and sums are read in fours.
+// 16-byte aligned: x, sums and v are read in fours.
 struct alignas(16) FewShared {
   union alignas(16) {
     float x[kGroup][kFewChunk];           // this block's part of the tokens' x
     float sums[kGroup][kFewThreads * 8];  // parts of up v
   };
   float part[kMaxRank][kGroup];  // its part of v, read by the whole cluster
-  float v[kMaxRank][kGroup];     // scale * v
+  alignas(16) float v[kMaxRank][kGroup];  // scale * v
   int tokens[kGroup];
   int count[kFewThreads / 32], n;
 };
+
+// Where column k of a token lies: lower and upper fours of the eights apart, so that the lanes' fours are neighbours.
+__device__ __forceinline__ int x_place(int k) { return (k & 4 ? kFewChunk / 2 : 0) + (k >> 3) * 4 + (k & 3); }
 
 // v parts of the rows of one adapter from `width` columns: a warp takes rows, LANES lanes a row.
 template <int NT, class W>
@@ -116,7 +119,7 @@ __device__ __forceinline__ void few_shrink(FewShared &sh, const W *down, int64_t
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) *reinterpret_cast<float4 *>(&x[t][e]) = *reinterpret_cast<const float4 *>(&sh.x[t][k + e]);
+        for (int e = 0; e < 8; e += 4) *reinterpret_cast<float4 *>(&x[t][e]) = *reinterpret_cast<const float4 *>(&sh.x[t][x_place(k + e)]);
 #pragma unroll
       for (int i = 0; i < B; ++i) {
         if (r0 + i * warps * rows >= rank) break;
@@ -173,12 +176,12 @@ __device__ __forceinline__ void few_expand(FewShared &sh, const sc_adapters_args
           if (r0 + i * sets >= rank) break;
           float f[8];
           w[i].get(f);
+          const float4 v4 = *reinterpret_cast<const float4 *>(sh.v[r0 + i * sets]);
+          const float v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const float v = sh.v[r0 + i * sets][t];
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[t][e] += f[e] * v;
-          }
+            for (int e = 0; e < 8; ++e) acc[t][e] += f[e] * v[t];
         }
       }
     __syncthreads();
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewBlocks) few_kernel(const __gr
     for (int g = 0; g < kGroup; ++g)
 #pragma unroll
       for (int i = 0; i < per; ++i)
-        if (tid + i * kFewThreads < wide) sh.x[g][tid + i * kFewThreads] = x[g][i];
+        if (tid + i * kFewThreads < wide) sh.x[g][x_place(tid + i * kFewThreads)] = x[g][i];
     __syncthreads();
     if (n == 1)
       few_shrink<1>(sh, down + k, s.in_row, rank, wide);
