@@ -63,8 +63,8 @@ __global__ void __launch_bounds__(256) pack_rows(const PackItem *list, W *dst) {
 // then each block makes its part of the rows of up v.  One launch, no scratch
 // memory.  Bound by latency (a chain of ids, weights, two cluster barriers,
 // weights) and fp32 instructions; the tensor-core tiles below have twice the
-// fixed cost: 128 tokens of 100 adapters of 512 x 2048 in bf16 take 15.4 us
-// here, 28.6 there; 96 tokens of 40 adapters of 4096 x 4096 22.7 and 33.3.
+// fixed cost: 128 tokens of 100 adapters of 512 x 2048 in bf16 take 14.8 us
+// here, 28.6 there; 96 tokens of 40 adapters of 4096 x 4096 21.4 and 33.3.
 constexpr int kFewTokens = 256, kGroup = 4 /* a float4 of v */, kFewChunk = 512, kFewThreads = 256, kFewBlocks = 3;
 
 // Eight weights, as they lie.
@@ -105,7 +105,8 @@ __device__ __forceinline__ void few_shrink(FewShared &sh, const W *down, int64_t
   int lanes = 32;
   while (lanes > 1 && lanes * 4 >= width) lanes >>= 1;
   const int sub = lane / lanes, in = lane % lanes, rows = 32 / lanes;
-  constexpr int B = 4, warps = kFewThreads / 32;  // B rows of a lane at a time
+  constexpr int B = 3, warps = kFewThreads / 32;  // B rows of a lane at a time (96 tokens of 40
+  // adapters of 4096 x 4096: 21.4 us with 3, 22.7 with 4, 21.7 with 6)
   for (int r0 = warp * rows; r0 < rank; r0 += B * warps * rows) {
     float acc[B][NT] = {};
     for (int k = in * 8; k < width; k += lanes * 8) {
