@@ -15,7 +15,9 @@ activations (features x tokens, fp32).  What a decoding step needs besides:
 
 Activations are fp32, fp16 or bf16 CUDA tensors with any strides; the cache is
 fp32, fp16 or bf16 of its own.  All calls are asynchronous on torch's current
-stream of the handle's device, or on ``stream``.  There is no CPU fallback.
+stream of the handle's device, or on ``stream``: that does not wait for the
+current one, and what the call allocates comes from its memory.  There is no
+CPU fallback.
 The reference (hosseinal/sparse-computation) ends at the products.
 """
 from __future__ import annotations
@@ -70,14 +72,24 @@ def _table(t, device: int) -> tuple:
     return t.data_ptr(), n, c, s
 
 
-def _on(stream, device: int, *tensors) -> int:
-    """The raw stream of a call on ``stream``; the tensors that it uses there are
-    kept from reuse until that stream is done with them."""
-    if stream.cuda_stream != _current(device):
-        for t in tensors:
-            if t is not None:
-                t.record_stream(stream)
-    return stream.cuda_stream
+def _on(stream, device: int, given, call):
+    """call() with ``stream`` current, so that outputs and scratch come from that stream's memory: a block that is free
+    on the stream that is current here may still have its last kernel ahead of it, and ``stream`` does not wait for
+    that.  The tensors of the call are kept from reuse until both streams are done with them."""
+    if stream.device.index != device:
+        _fail(f"the stream is on {stream.device}, the call on cuda:{device}")
+    here = torch.cuda.current_stream(device)
+    if stream == here:
+        return call()
+    with torch.cuda.stream(stream):
+        got = call()
+    for t in given:
+        if t is not None:
+            t.record_stream(stream)
+    for t in got if isinstance(got, tuple) else (got,):
+        if t is not None:
+            t.record_stream(here)
+    return got
 
 
 # torch.cuda.current_stream builds an object (1.2 us a call); the raw handle is all that a launch needs.
@@ -177,6 +189,10 @@ class PagedKVCache(_Handle):
         token with a negative position is skipped: nothing is stored, its q
         rows become zero.  positions, seq_ids and page_table are int32."""
         dev, dtype = self.device, k.dtype
+        if stream is not None:
+            return _on(stream, dev, (k, v, positions, seq_ids, page_table, q, q_out, self.k, self.v,
+                                     *((rope.cos, rope.sin) if rope is not None else ())),
+                       lambda: self.append(k, v, positions, page_table, seq_ids, rope, q, q_out))
         kind = _TYPES.get(dtype)
         if kind is None or k.dim() != 3:
             _fail("k must be a 3-D float32, float16 or bfloat16 tensor")
@@ -215,10 +231,8 @@ class PagedKVCache(_Handle):
             if n:
                 _fail("an empty page table")
             return q_out
-        s = _current(dev) if stream is None else _on(stream, dev, k, v, positions, seq_ids, page_table, q, q_out, self.k,
-                                                     self.v, *((rope.cos, rope.sin) if rope is not None else ()))
         bad = self._call(self._h, _APPEND.pack(n, heads, kind, *ka, *va, *qa, *oa, pos, ids, tab, seqs, cols, tstride,
-                                               *ra), s)
+                                               *ra), _current(dev))
         if bad:
             _check(bad)
         return q_out
@@ -254,6 +268,9 @@ class DecodeAttention(_Handle):
         out: [seqs, q_heads, head_dim] of one type.  A sequence of length 0
         gives zeros (lse -inf).  Returns out, or (out, lse [seqs, q_heads])."""
         dev, dtype = self.device, q.dtype
+        if stream is not None:
+            return _on(stream, dev, (q, page_table, seq_lens, out, self.cache.k, self.cache.v, self._work),
+                       lambda: self.attend(q, page_table, seq_lens, out, return_lse))
         kind = _TYPES.get(dtype)
         if kind is None or q.dim() != 3:
             _fail("q must be a 3-D float32, float16 or bfloat16 tensor")
@@ -274,10 +291,8 @@ class DecodeAttention(_Handle):
         lens = _ints(seq_lens, "seq_lens", dev, n)
         lse = q.new_empty((n, self.q_heads), dtype=torch.float32) if return_lse else None
         if n:
-            s = _current(dev) if stream is None else _on(stream, dev, q, out, page_table, seq_lens, lse, self.cache.k,
-                                                         self.cache.v, self._work)
             bad = self._call(self._h, _ATTEND.pack(n, kind, *qa, *oa, lse.data_ptr() if return_lse else 0, tab, cols,
-                                                   tstride, lens), s)
+                                                   tstride, lens), _current(dev))
             if bad:
                 _check(bad)
         return (out, lse) if return_lse else out
@@ -339,6 +354,8 @@ class LowRankAdapters(_Handle):
         type with any strides, as SpMMPlan.spmm's B and C; ids [tokens] int32,
         negative for a token without an adapter.  out may be base."""
         dev, dtype = self.device, x.dtype
+        if stream is not None:
+            return _on(stream, dev, (x, ids, base, out, self._memory), lambda: self.apply(x, ids, base, out))
         kind = _TYPES.get(dtype)
         if kind is None or x.dim() != 2:
             _fail("x must be a 2-D float32, float16 or bfloat16 tensor")
@@ -361,8 +378,8 @@ class LowRankAdapters(_Handle):
         if n:
             size = self._workspace(n)
             work = x.new_empty(size, dtype=torch.uint8) if size else None
-            s = _current(dev) if stream is None else _on(stream, dev, x, ids, base, out, work, self._memory)
-            bad = self._call(self._h, _ADAPT.pack(n, kind, *xa, *ba, *oa, idp, work.data_ptr() if size else 0, size), s)
+            bad = self._call(self._h, _ADAPT.pack(n, kind, *xa, *ba, *oa, idp, work.data_ptr() if size else 0, size),
+                             _current(dev))
             if bad:
                 _check(bad)
         return out

@@ -1,0 +1,159 @@
+"""Serving operators and streams: where a call's memory comes from, and how long it is kept.
+
+The host side runs on the CPU with a recorder in place of CUDA's streams and of
+the library; the GPU tests run the same situations."""
+import contextlib
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+import serving_ref as ref
+import sparse_computation_b200 as sc
+from sparse_computation_b200 import serving
+
+
+class Stream:
+    def __init__(self, raw):
+        self.cuda_stream, self.device = raw, SimpleNamespace(index=-1)
+
+
+MAIN, SIDE = Stream(1), Stream(2)
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    """Streams without a GPU (CPU tensors are on device -1): ``made`` lists (raw stream, tensor) of what calls
+    allocate, ``kept`` (raw stream, data pointer) of record_stream, ``launched`` the raw streams of the C calls."""
+    log = SimpleNamespace(now=MAIN, made=[], kept=[], launched=[])
+
+    @contextlib.contextmanager
+    def current(stream):
+        before, log.now = log.now, stream
+        yield
+        log.now = before
+
+    new_empty = torch.Tensor.new_empty
+
+    def allocate(self, *shape, **kw):
+        t = new_empty(self, *shape, **kw)
+        log.made.append((log.now.cuda_stream, t))
+        return t
+
+    monkeypatch.setattr(torch.Tensor, "new_empty", allocate)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: log.kept.append((s.cuda_stream, t.data_ptr())),
+                        raising=False)
+    monkeypatch.setattr(torch.cuda, "stream", current)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: log.now)
+    monkeypatch.setattr(serving, "_current", lambda device: log.now.cuda_stream)
+    return log
+
+
+def handle(log, cls, **fields):
+    """A handle of ``cls`` without the library behind it."""
+    h = cls.__new__(cls)
+    h.device = -1
+    h._call = lambda handle, args, stream: log.launched.append(stream)
+    for name, value in fields.items():
+        setattr(h, name, value)
+    return h
+
+
+def calls(log):
+    """name -> (a call with stream=..., its tensors), for each operator; tokens enough for scratch."""
+    n, h, d = 300, 2, 8
+    x = torch.zeros(n, h, d)
+    ints, table = torch.zeros(n, dtype=torch.int32), torch.zeros(n, 1, dtype=torch.int32)
+    cache = handle(log, sc.PagedKVCache, k=torch.zeros(4, h, 4, d), v=torch.zeros(4, h, 4, d), kv_heads=h, head_dim=d)
+    plan = handle(log, sc.DecodeAttention, cache=cache, q_heads=h, max_seqs=n, _work=torch.zeros(64, dtype=torch.uint8))
+    adapters = handle(log, sc.LowRankAdapters, in_features=8, out_features=6, _memory=torch.zeros(64, dtype=torch.uint8))
+    adapters._scratch = (n, 128)
+    cols = torch.zeros(8, n)
+    return {
+        "append": (lambda **kw: cache.append(x, x, ints, table, q=x, **kw), [x, ints, table, cache.k, cache.v]),
+        "attend": (lambda **kw: plan.attend(x, table, ints, return_lse=True, **kw),
+                   [x, table, ints, cache.k, cache.v, plan._work]),
+        "apply": (lambda **kw: adapters.apply(cols, ints, **kw), [cols, ints, adapters._memory]),
+    }
+
+
+@pytest.mark.parametrize("name,allocations", [("append", 1), ("attend", 2), ("apply", 2)])
+def test_a_call_on_another_stream_allocates_there(recorder, name, allocations):
+    """Outputs and scratch of a call with stream= come from that stream's memory, and outputs are kept for the stream
+    that was current; its inputs are kept for the stream that reads them."""
+    call, given = calls(recorder)[name]
+    got = call(stream=SIDE)
+    assert recorder.launched == [SIDE.cuda_stream] and recorder.now is MAIN
+    assert [raw for raw, _ in recorder.made] == [SIDE.cuda_stream] * allocations
+    for t in given:
+        assert (SIDE.cuda_stream, t.data_ptr()) in recorder.kept
+    for t in got if isinstance(got, tuple) else (got,):
+        assert (MAIN.cuda_stream, t.data_ptr()) in recorder.kept
+
+
+@pytest.mark.parametrize("name", ["append", "attend", "apply"])
+def test_a_call_on_the_current_stream_records_nothing(recorder, name):
+    call, _ = calls(recorder)[name]
+    for kw in ({}, {"stream": MAIN}):
+        recorder.launched.clear()
+        call(**kw)
+        assert recorder.launched == [MAIN.cuda_stream] and not recorder.kept
+
+
+@pytest.mark.parametrize("name", ["append", "attend", "apply"])
+def test_a_stream_of_another_device_is_refused(recorder, name):
+    call, _ = calls(recorder)[name]
+    other = Stream(3)
+    other.device = SimpleNamespace(index=1)
+    with pytest.raises(sc.ScError) as e:
+        call(stream=other)
+    assert e.value.code == sc.SC_ERR_ARG and not recorder.launched
+
+
+# -------------------------------------------------------------------- GPU --
+
+@pytest.mark.gpu
+def test_adapters_of_two_streams_do_not_share_scratch(cuda):
+    """Batches of different size and order on the current stream and on another one, without a wait between them."""
+    gen = torch.Generator().manual_seed(20)
+    down = [torch.randn(8, 256, generator=gen) / 16 for _ in range(3)]
+    up = [torch.randn(128, 8, generator=gen) / 3 for _ in range(3)]
+    s = sc.LowRankAdapters([a.cuda() for a in down], [b.cuda() for b in up], [1.0, 0.5, 2.0])
+    batches = []
+    for n in (2000, 300):
+        x, ids = torch.randn(256, n, generator=gen), torch.randint(-1, 3, (n,), generator=gen).int()
+        batches.append((x.cuda(), ids.cuda(), *ref.adapters(x, ids, down, up, [1.0, 0.5, 2.0], None, torch.float32)))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        got.append((s.apply(*batches[0][:2]), s.apply(*batches[1][:2], stream=side)))
+    torch.cuda.synchronize()
+    s.check()
+    for pair in got:
+        for y, (_, _, want, tol) in zip(pair, batches):
+            assert ((y.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+def test_outputs_on_another_stream_take_no_block_of_the_current_one(cuda):
+    """A block freed on the current stream, whose last kernel is still ahead, is not what the other stream's output gets."""
+    cache = sc.PagedKVCache.allocate(4, 16, 2, 64)
+    plan = sc.DecodeAttention(cache, 2, 300)
+    s = sc.LowRankAdapters([torch.ones(4, 256, device=cuda)], [torch.ones(128, 4, device=cuda)], [1.0])
+    q, table = torch.ones(300, 2, 64, device=cuda), torch.zeros(300, 4, dtype=torch.int32, device=cuda)
+    ids, x = torch.zeros(300, dtype=torch.int32, device=cuda), torch.ones(256, 300, device=cuda)
+    side = torch.cuda.Stream()
+    for call in (lambda: cache.append(q[:4], q[:4], ids[:4] - 1, table, q=q[:4], stream=side),
+                 lambda: plan.attend(q, table, ids, stream=side),
+                 lambda: s.apply(x, ids, stream=side)):
+        size = call().numel()
+        torch.cuda.synchronize()
+        freed = torch.empty(size, device=cuda)
+        torch.cuda._sleep(20_000_000)  # about 10 ms
+        freed.add_(1)
+        at = freed.data_ptr()
+        del freed
+        out = call()
+        assert not at <= out.data_ptr() < at + 4 * size
+        torch.cuda.synchronize()
