@@ -118,10 +118,23 @@ class _Handle:
         if v:
             raise ScError(SC_ERR_DEVICE, f"a kernel skipped entries that were out of range (status {v})")
 
-    def _own(self, h: ctypes.c_void_p) -> None:
+    def _own(self, h: ctypes.c_void_p, *memory) -> None:
+        """``memory``: device tensors that only the handle keeps alive.  They come from the stream that is current now."""
         self._h = h
+        self._kept, self._streams = memory, {_current(self.device)}
         self._release = getattr(lib(), self._free)  # module globals may be gone when the interpreter ends
         self._call = getattr(lib(), self._run)
+
+    def _stream(self) -> int:
+        """The raw current stream, for a launch.  The handle's memory is kept from reuse until that stream is done with
+        it, however early the handle is dropped; once for each stream is enough, as the allocator looks when it is
+        freed."""
+        raw = _current(self.device)
+        if raw not in self._streams:
+            for t in self._kept:
+                t.record_stream(torch.cuda.current_stream(self.device))
+            self._streams.add(raw)
+        return raw
 
     def __del__(self):
         if self._h is not None:
@@ -170,7 +183,7 @@ class PagedKVCache(_Handle):
                           *k.stride()[:3], *v.stride()[:3], _TYPES[k.dtype])
         h = ctypes.c_void_p()
         _check(lib().sc_kv_cache_create(pool, self.device, ctypes.byref(h)))
-        self._own(h)
+        self._own(h, k, v)
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.float32,
@@ -190,7 +203,7 @@ class PagedKVCache(_Handle):
         rows become zero.  positions, seq_ids and page_table are int32."""
         dev, dtype = self.device, k.dtype
         if stream is not None:
-            return _on(stream, dev, (k, v, positions, seq_ids, page_table, q, q_out, self.k, self.v,
+            return _on(stream, dev, (k, v, positions, seq_ids, page_table, q, q_out,
                                      *((rope.cos, rope.sin) if rope is not None else ())),
                        lambda: self.append(k, v, positions, page_table, seq_ids, rope, q, q_out))
         kind = _TYPES.get(dtype)
@@ -232,7 +245,7 @@ class PagedKVCache(_Handle):
                 _fail("an empty page table")
             return q_out
         bad = self._call(self._h, _APPEND.pack(n, heads, kind, *ka, *va, *qa, *oa, pos, ids, tab, seqs, cols, tstride,
-                                               *ra), _current(dev))
+                                               *ra), self._stream())
         if bad:
             _check(bad)
         return q_out
@@ -260,7 +273,7 @@ class DecodeAttention(_Handle):
         torch.cuda.current_stream(self.device).synchronize()  # whatever used that memory before is done
         at = (self._work.data_ptr() + 255) // 256 * 256
         _check(lib().sc_attn_create_in(cache._h, q_heads, max_seqs, scale or 0.0, window, at, size.value, ctypes.byref(h)))
-        self._own(h)
+        self._own(h, self._work, cache.k, cache.v)
 
     def attend(self, q, page_table, seq_lens, out=None, return_lse: bool = False, stream=None):
         """out[s] = softmax(scale q[s] k^T) v over the ``seq_lens[s]`` first
@@ -269,7 +282,7 @@ class DecodeAttention(_Handle):
         gives zeros (lse -inf).  Returns out, or (out, lse [seqs, q_heads])."""
         dev, dtype = self.device, q.dtype
         if stream is not None:
-            return _on(stream, dev, (q, page_table, seq_lens, out, self.cache.k, self.cache.v, self._work),
+            return _on(stream, dev, (q, page_table, seq_lens, out),
                        lambda: self.attend(q, page_table, seq_lens, out, return_lse))
         kind = _TYPES.get(dtype)
         if kind is None or q.dim() != 3:
@@ -292,7 +305,7 @@ class DecodeAttention(_Handle):
         lse = q.new_empty((n, self.q_heads), dtype=torch.float32) if return_lse else None
         if n:
             bad = self._call(self._h, _ATTEND.pack(n, kind, *qa, *oa, lse.data_ptr() if return_lse else 0, tab, cols,
-                                                   tstride, lens), _current(dev))
+                                                   tstride, lens), self._stream())
             if bad:
                 _check(bad)
         return (out, lse) if return_lse else out
@@ -337,7 +350,7 @@ class LowRankAdapters(_Handle):
             self.device, self.in_features, self.out_features, n, r, _TYPES[dtype],
             vp(*[a.data_ptr() for a in down]), i64(*dl), vp(*[b.data_ptr() for b in up]), i64(*ul),
             (ctypes.c_float * n)(*[float(x) for x in scales]), _current(self.device), at, size.value, ctypes.byref(h)))
-        self._own(h)
+        self._own(h, self._memory)
         self.ranks = ranks
         self._scratch = (-1, 0)
 
@@ -355,7 +368,7 @@ class LowRankAdapters(_Handle):
         negative for a token without an adapter.  out may be base."""
         dev, dtype = self.device, x.dtype
         if stream is not None:
-            return _on(stream, dev, (x, ids, base, out, self._memory), lambda: self.apply(x, ids, base, out))
+            return _on(stream, dev, (x, ids, base, out), lambda: self.apply(x, ids, base, out))
         kind = _TYPES.get(dtype)
         if kind is None or x.dim() != 2:
             _fail("x must be a 2-D float32, float16 or bfloat16 tensor")
@@ -379,7 +392,7 @@ class LowRankAdapters(_Handle):
             size = self._workspace(n)
             work = x.new_empty(size, dtype=torch.uint8) if size else None
             bad = self._call(self._h, _ADAPT.pack(n, kind, *xa, *ba, *oa, idp, work.data_ptr() if size else 0, size),
-                             _current(dev))
+                             self._stream())
             if bad:
                 _check(bad)
         return out

@@ -49,13 +49,14 @@ def recorder(monkeypatch):
     return log
 
 
-def handle(log, cls, **fields):
+def handle(log, cls, kept=(), **fields):
     """A handle of ``cls`` without the library behind it."""
     h = cls.__new__(cls)
     h.device = -1
     h._call = lambda handle, args, stream: log.launched.append(stream)
     for name, value in fields.items():
         setattr(h, name, value)
+    h._kept, h._streams = tuple(kept), {MAIN.cuda_stream}
     return h
 
 
@@ -64,9 +65,10 @@ def calls(log):
     n, h, d = 300, 2, 8
     x = torch.zeros(n, h, d)
     ints, table = torch.zeros(n, dtype=torch.int32), torch.zeros(n, 1, dtype=torch.int32)
-    cache = handle(log, sc.PagedKVCache, k=torch.zeros(4, h, 4, d), v=torch.zeros(4, h, 4, d), kv_heads=h, head_dim=d)
-    plan = handle(log, sc.DecodeAttention, cache=cache, q_heads=h, max_seqs=n, _work=torch.zeros(64, dtype=torch.uint8))
-    adapters = handle(log, sc.LowRankAdapters, in_features=8, out_features=6, _memory=torch.zeros(64, dtype=torch.uint8))
+    pools, work, memory = torch.zeros(2, 4, h, 4, d), torch.zeros(64, dtype=torch.uint8), torch.zeros(64, dtype=torch.uint8)
+    cache = handle(log, sc.PagedKVCache, pools, k=pools[0], v=pools[1], kv_heads=h, head_dim=d)
+    plan = handle(log, sc.DecodeAttention, (work, *pools), cache=cache, q_heads=h, max_seqs=n, _work=work)
+    adapters = handle(log, sc.LowRankAdapters, (memory,), in_features=8, out_features=6, _memory=memory)
     adapters._scratch = (n, 128)
     cols = torch.zeros(8, n)
     return {
@@ -98,6 +100,26 @@ def test_a_call_on_the_current_stream_records_nothing(recorder, name):
         recorder.launched.clear()
         call(**kw)
         assert recorder.launched == [MAIN.cuda_stream] and not recorder.kept
+
+
+@pytest.mark.parametrize("name,owned", [("append", slice(3, 5)), ("attend", slice(3, 6)), ("apply", slice(2, 3))])
+@pytest.mark.parametrize("explicit", [False, True])
+def test_memory_of_a_handle_is_kept_for_every_stream_it_is_used_on(recorder, name, owned, explicit):
+    """Under torch.cuda.stream(side) as with stream=side: dropping the handle then gives nothing back that side's
+    kernels still use."""
+    call, given = calls(recorder)[name]
+    if explicit:
+        call(stream=SIDE)
+    else:
+        with torch.cuda.stream(SIDE):
+            call()
+    for t in given[owned]:
+        assert (SIDE.cuda_stream, t.data_ptr()) in recorder.kept
+    recorder.kept.clear()
+    with torch.cuda.stream(SIDE):
+        call()
+    assert recorder.launched == [SIDE.cuda_stream] * 2
+    assert not recorder.kept  # the allocator remembers a stream until the memory is freed
 
 
 @pytest.mark.parametrize("name", ["append", "attend", "apply"])
@@ -133,6 +155,43 @@ def test_adapters_of_two_streams_do_not_share_scratch(cuda):
     for pair in got:
         for y, (_, _, want, tol) in zip(pair, batches):
             assert ((y.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("explicit", [False, True])
+def test_a_dropped_handle_keeps_its_memory_until_its_streams_are_done(cuda, explicit):
+    side = torch.cuda.Stream()
+    q, table = torch.ones(4, 2, 64, device=cuda), torch.zeros(4, 4, dtype=torch.int32, device=cuda)
+    ids, x = torch.zeros(4, dtype=torch.int32, device=cuda), torch.ones(256, 4, device=cuda)
+    torch.cuda.synchronize()
+
+    def use(call):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)  # about 10 ms
+            if not explicit:
+                return call()
+        return call(stream=side)
+
+    cache = sc.PagedKVCache.allocate(4, 16, 2, 64)
+
+    def plan():
+        p = sc.DecodeAttention(cache, 2, 4)
+        use(lambda **kw: p.attend(q, table, ids, **kw))
+        return p._work
+
+    def adapters():
+        s = sc.LowRankAdapters([torch.ones(64, 256, device=cuda)], [torch.ones(1000, 64, device=cuda)], [1.0])
+        use(lambda **kw: s.apply(x, ids, **kw))
+        return s._memory
+
+    for make in (plan, adapters):
+        t = make()  # the handle is gone when this returns
+        at, n = t.data_ptr(), t.numel()
+        del t
+        again = torch.empty(n, dtype=torch.uint8, device=cuda)
+        assert not side.query()  # or the test shows nothing
+        assert not at <= again.data_ptr() < at + n
+        torch.cuda.synchronize()
 
 
 @pytest.mark.gpu
