@@ -355,11 +355,13 @@ class LowRankAdapters(_Handle):
         self._scratch = (-1, 0)
 
     def _workspace(self, n: int) -> int:
-        if self._scratch[0] != n:
+        tokens, size = self._scratch  # read once: another thread may put its own pair there
+        if tokens != n:
             b = ctypes.c_int64()
             _check(lib().sc_adapters_workspace(self._h, n, ctypes.byref(b)))
-            self._scratch = (n, b.value)
-        return self._scratch[1]
+            size = b.value
+            self._scratch = (n, size)
+        return size
 
     def apply(self, x, ids, base=None, out=None, stream=None):
         """out = base + the adapters' part of each token: x [in_features,

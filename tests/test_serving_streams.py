@@ -132,6 +132,29 @@ def test_a_stream_of_another_device_is_refused(recorder, name):
     assert e.value.code == sc.SC_ERR_ARG and not recorder.launched
 
 
+def test_scratch_sizes_of_two_threads_stay_apart(recorder, monkeypatch):
+    """Another thread's call with more tokens between any two steps of a size lookup does not change its answer."""
+    class Shared(sc.LowRankAdapters):
+        stored = (-1, 0)
+
+        @property
+        def _scratch(self):
+            return self.stored
+
+        @_scratch.setter
+        def _scratch(self, pair):
+            self.stored = (999, 999 * 8)  # the other thread's, put there right after ours
+
+    def size(h, n, out):
+        out._obj.value = n * 8
+        return 0
+
+    monkeypatch.setattr(serving, "lib", lambda: SimpleNamespace(sc_adapters_workspace=size))
+    s = handle(recorder, Shared)
+    s._h = None
+    assert [s._workspace(n) for n in (300, 400, 999)] == [300 * 8, 400 * 8, 999 * 8]
+
+
 # -------------------------------------------------------------------- GPU --
 
 @pytest.mark.gpu
