@@ -208,6 +208,8 @@ def test_a_dropped_handle_keeps_its_memory_until_its_streams_are_done(cuda, expl
         return s._memory
 
     for make in (plan, adapters):
+        make()  # loads the kernels
+        torch.cuda.synchronize()
         t = make()  # the handle is gone when this returns
         at, n = t.data_ptr(), t.numel()
         del t
@@ -229,7 +231,7 @@ def test_outputs_on_another_stream_take_no_block_of_the_current_one(cuda):
     for call in (lambda: cache.append(q[:4], q[:4], ids[:4] - 1, table, q=q[:4], stream=side),
                  lambda: plan.attend(q, table, ids, stream=side),
                  lambda: s.apply(x, ids, stream=side)):
-        size = call().numel()
+        size = call().numel()  # and loads the kernels
         torch.cuda.synchronize()
         freed = torch.empty(size, device=cuda)
         torch.cuda._sleep(20_000_000)  # about 10 ms
