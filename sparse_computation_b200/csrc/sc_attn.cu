@@ -82,8 +82,7 @@ std::unique_ptr<sc_attn> set_up(const sc_kv_cache *cache, int64_t q_heads, int64
 }
 
 void give_workspace(sc_attn &p, void *at, const Layout &layout) {
-  cuda_check(cudaMemset(at, 0, layout.words * 4), "clear attention workspace");
-  cuda_check(cudaStreamSynchronize(nullptr), "stream synchronize");
+  clear_words(at, layout.words * 4);
   p.status = static_cast<int *>(at);
   p.arrivals = p.status + 64 + 256;
   p.heads = reinterpret_cast<float *>(p.status + layout.words);

@@ -472,8 +472,7 @@ int sc_kv_cache_create(const sc_kv_pool *pool, int32_t device, sc_kv_cache **out
   c->pool = *pool;
   c->device = device;
   DeviceGuard dg(device);
-  c->status.alloc(device, 256, "allocate status word");
-  cuda_check(cudaMemset(c->status.p, 0, 256), "clear status word");
+  make_status(c->status, device);
   *out = c.release();
   SC_SERVE_END
 }

@@ -56,14 +56,28 @@ struct DeviceBlock {
   }
 };
 
+// Zeros at p when this returns.  The wait matters: the memset is asynchronous on
+// the legacy stream, and a kernel that a non-blocking stream starts next could
+// set a status before it.
+inline void clear_words(void *p, size_t bytes) {
+  cuda_check(cudaMemset(p, 0, bytes), "clear status");
+  cuda_check(cudaStreamSynchronize(nullptr), "stream synchronize");
+}
+
 // Reads and clears a device status word after all work on its device.
 inline int take_status(int device, int *word) {
   DeviceGuard dg(device);
   cuda_check(cudaDeviceSynchronize(), "device synchronize");
   int v = 0;
   cuda_check(cudaMemcpy(&v, word, sizeof v, cudaMemcpyDeviceToHost), "read status");
-  if (v) cuda_check(cudaMemset(word, 0, sizeof v), "clear status");
+  if (v) clear_words(word, sizeof v);
   return v;
+}
+
+// A cleared status word of its own, on the current device.
+inline void make_status(DeviceBlock &block, int device) {
+  block.alloc(device, 256, "allocate status word");
+  clear_words(block.p, 256);
 }
 
 inline int64_t type_bytes(int64_t t) { return t == SC_TYPE_F32 ? 4 : 2; }
