@@ -592,4 +592,17 @@ class Graph:
             self._h = ctypes.c_void_p()
 
 
-from .serving import DecodeAttention, LowRankAdapters, PagedKVCache, RotaryTable  # noqa: E402,F401
+_SERVING = ("DecodeAttention", "LowRankAdapters", "PagedKVCache", "RotaryTable")
+
+
+def __getattr__(name: str):
+    # The serving operators need torch, whose import takes ten times as long as everything else here.
+    if name in _SERVING:
+        from . import serving
+        globals().update({n: getattr(serving, n) for n in _SERVING})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted({*globals(), *_SERVING})
