@@ -336,8 +336,9 @@ class LowRankAdapters(_Handle):
             if a.shape[1] != self.in_features or b.shape[0] != self.out_features or a.shape[0] != b.shape[1]:
                 _fail(f"adapter shapes do not match: down {tuple(a.shape)}, up {tuple(b.shape)}")
             ranks.append(a.shape[0])
-        down = [a if a.stride(1) == 1 else a.contiguous() for a in down]
-        up = [b if b.stride(1) == 1 else b.contiguous() for b in up]
+        # rows that lie apart, as the packing reads them; expanded or overlapping ones are copied first
+        plain = lambda w: w if w.stride(1) == 1 and (w.shape[0] == 1 or w.stride(0) >= w.shape[1]) else w.contiguous()
+        down, up = [plain(a) for a in down], [plain(b) for b in up]
         i64, vp = ctypes.c_int64 * n, ctypes.c_void_p * n
         # a single row's stride means nothing: give the row length
         dl = [a.stride(0) if a.shape[0] > 1 else max(a.shape[1], 1) for a in down]
