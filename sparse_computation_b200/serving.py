@@ -324,6 +324,8 @@ class LowRankAdapters(_Handle):
         if n == 0 or len(up) != n or len(scales) != n:
             _fail("down, up and scales must be non-empty lists of one length")
         dtype, where = down[0].dtype, down[0].device
+        if down[0].dim() != 2 or up[0].dim() != 2:
+            _fail("adapter weights must be 2-D, of one type and on one device")
         if dtype not in _TYPES or where.type != "cuda":
             _fail("adapter weights must be float32, float16 or bfloat16 CUDA tensors")
         self.in_features, self.out_features = down[0].shape[-1], up[0].shape[0]

@@ -27,3 +27,11 @@ def test_adapter_weights_may_be_expanded_or_overlap(cuda):
     got = s.apply(x.cuda(), ids.cuda())
     want, tol = ref.adapters(x, ids, down, up, [1.0, -0.5, 2.0], None, F32)
     assert ((got.cpu().double() - want).abs() <= tol).all()
+
+
+def test_refusals_of_weights_without_two_dimensions(cuda):
+    w = torch.zeros(4, 8, device=cuda)
+    for down, up in ((torch.zeros((), device=cuda), w.t()), (w, torch.zeros((), device=cuda)), (w, torch.zeros(8, device=cuda))):
+        with pytest.raises(sc.ScError) as e:
+            sc.LowRankAdapters([down], [up], [1.0])
+        assert e.value.code == sc.SC_ERR_ARG
