@@ -104,6 +104,9 @@ struct Cfg {
   // bf16 batch / of windows over fp16: 38.6 69.7 28.7 with 1, 39.9 65.5 26.4 with 2, 40.8 62.7 26.1 with 3, 42.1 61.9
   // 26.9 with 4.
   static constexpr int change = f32 ? 1 : 3;
+  // P (1 at most) as it is split into fp16 parts: two parts then keep weights down to 2^-38 of the largest, where fp16's
+  // smallest value would cut those of e^-16 to a single bit.  Taken off again where a portion's result is written.
+  static constexpr float lift = is_f16(MODE) ? 16384.f : 1.f;
   static constexpr bool ahead = DP <= 128;                   // registers suffice to load K a phase ahead
   static constexpr int o_row = DP + 4;                       // floats; the pad spreads rows over the banks
   static constexpr int piece = kQT * o_row + 2 * kQT;        // O | m | l
@@ -619,6 +622,7 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
         for (int e = 0; e < 2; ++e) {
           x[nt][e] = ex2(fmaf(x[nt][e], c, -ref));
           l += x[nt][e];
+          x[nt][e] *= C::lift;
         }
       constexpr int PN = C::f32 ? C::NT : C::NT / 2;  // A fragments of P: of 8 keys (f32) or 16
       uint32_t pa[PN][4], p3[PN][2];
@@ -700,7 +704,8 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
 #pragma unroll
         for (int e = 0; e < C::epc; e += 4) {
           const int d = (8 * j + 2 * t + k) * C::epc + e, b = j * C::epc + e;
-          float4 y = make_float4(o[b][k], o[b + 1][k], o[b + 2][k], o[b + 3][k]);
+          constexpr float down = 1.f / C::lift;
+          float4 y = make_float4(o[b][k] * down, o[b + 1][k] * down, o[b + 2][k] * down, o[b + 3][k] * down);
           if (C::quarter) {
             y.x += __shfl_xor_sync(~0u, y.x, 16);
             y.y += __shfl_xor_sync(~0u, y.y, 16);
