@@ -486,9 +486,7 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
         }
       }
     };
-    // fp16 parts: a row is scaled by a power of two to below 2, so that no part overflows and the tails stay above
-    // fp16's smallest values
-    float up = 1.f;
+    float up = 1.f;  // fp16 parts are of scaled rows
     if (MODE == kF16Wide) {
       float top = 0.f;
 #pragma unroll 1
@@ -500,8 +498,7 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
       }
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-      const int e = (int)(__float_as_uint(top) >> 23) - 127;  // floor(log2(top)) of a normal number
-      if (e > -120 && e < 127) up = __uint_as_float((uint32_t)(e + 127) << 23);
+      up = f16_scale(top);
     }
     c = p.scale_log2 * up;
 #pragma unroll 1

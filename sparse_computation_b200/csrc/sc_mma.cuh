@@ -37,6 +37,15 @@ __device__ __forceinline__ uint32_t tf32_tail(float x) {
   return __float_as_uint(x - __uint_as_float(__float_as_uint(x) & 0xffffe000u));
 }
 
+// The power of two that brings a row of largest value `top` to below 2^15 for a
+// split into two fp16 parts: no part overflows, and values down to 2^-40 of the
+// largest are not lost below fp16's smallest.  Rows below 2^-112 are brought up
+// by no more than 2^126, so that the inverse is a normal number too.
+__device__ __forceinline__ float f16_scale(float top) {
+  const int e = (int)(__float_as_uint(top) >> 23) - 127;  // floor(log2(top)) of a normal number; 128: not finite
+  return e < 128 ? __uint_as_float((uint32_t)((e > -112 ? e : -112) - 14 + 127) << 23) : 1.f;
+}
+
 // Two floats as packed 16-bit values, and what the packing lost of them.
 template <int MODE>
 __device__ __forceinline__ uint32_t pack2(float &a, float &b) {

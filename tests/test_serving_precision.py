@@ -50,3 +50,14 @@ def test_weights_far_below_a_sink(cuda, kind, stored, n):
     k[0, :, 5] = (x * (16 * 8 / x.square().sum(-1, keepdim=True))).to(stored)
     v[0, :, 5] = 0
     held(*attention(q, k, v, [n], page))
+
+
+@pytest.mark.parametrize("kind,stored", WIDE)
+def test_a_query_with_an_outlier_that_meets_zeros(cuda, kind, stored):
+    gen = torch.Generator().manual_seed(41)
+    d, page = 64, 16
+    k, v = (torch.randn(3, 2, page, d, generator=gen).to(stored) for _ in range(2))
+    q = torch.randn(1, 4, d, generator=gen).to(kind)
+    q[:, :, 9] = 2.0 ** 18
+    k[..., 9] = 0
+    held(*attention(q, k, v, [40], page))
