@@ -356,12 +356,6 @@ struct Kind {
   static constexpr bool scaled = f16 && !same;
 };
 
-// The power of two that brings top to below 2.
-__device__ __forceinline__ float scale_to_two(float top) {
-  const int e = (int)(__float_as_uint(top) >> 23) - 127;
-  return e > -120 && e < 127 ? __uint_as_float((uint32_t)(e + 127) << 23) : 1.f;
-}
-
 // Two neighbouring values of rows g and g + 8 as parts of A: a[part][0] row g, [1] row g + 8.
 template <int MODE, int PARTS>
 __device__ __forceinline__ void split2(float x0, float x1, float y0, float y1, uint32_t (&a)[PARTS][2]) {
@@ -502,8 +496,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
           top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
         }
-        up_g = scale_to_two(top[0]);
-        up_g8 = scale_to_two(top[1]);
+        up_g = mma::f16_scale(top[0]);
+        up_g8 = mma::f16_scale(top[1]);
 #pragma unroll
         for (int j = 0; j < K::J; ++j)
 #pragma unroll
@@ -613,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int r = t; r < rank; r += 4) top = fmaxf(top, fabsf(v[(g + 8 * h) * v_row + r]));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-      vs[h] = scale_to_two(top);
+      vs[h] = mma::f16_scale(top);
     }
   }
   const float vi[2] = {1.f / vs[0], 1.f / vs[1]};

@@ -61,3 +61,29 @@ def test_a_query_with_an_outlier_that_meets_zeros(cuda, kind, stored):
     q[:, :, 9] = 2.0 ** 18
     k[..., 9] = 0
     held(*attention(q, k, v, [40], page))
+
+
+ADAPTERS = [(F32, F32), (F32, BF16), (F32, F16), (BF16, F16)]
+
+
+@pytest.mark.parametrize("kind,stored", ADAPTERS)
+@pytest.mark.parametrize("tokens", [40, 300])
+@pytest.mark.parametrize("where", ["x", "v"])
+def test_adapters_with_an_outlier_that_meets_zeros(cuda, kind, stored, tokens, where):
+    """A feature of x that `down` does not read, or a rank that `up` does not read, 2^14 times larger than the others."""
+    gen = torch.Generator().manual_seed(42)
+    k, m, r = 64, 72, 12
+    down, up = (torch.randn(r, k, generator=gen) / 8).to(stored), (torch.randn(m, r, generator=gen) / 3).to(stored)
+    x = torch.randn(k, tokens, generator=gen).to(kind)
+    if where == "x":
+        x[7] = 2.0 ** 14
+        down[:, 7] = 0
+    else:
+        down[3] = 2.0 ** 14 * torch.sign(down[3].float()).to(stored)
+        x[:] = x.abs() * torch.sign(down[3].float()).to(kind)[:, None]
+        up[:, 3] = 0
+    s = sc.LowRankAdapters([down.cuda()], [up.cuda()], [1.0])
+    ids = torch.zeros(tokens, dtype=torch.int32)
+    got = s.apply(x.cuda(), ids.cuda()).cpu().double()
+    want, tol = ref.adapters(x, ids, [down], [up], [1.0], None, kind)
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
