@@ -324,7 +324,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewBlocks) few_kernel(const __gr
 // result): of `down`, piece t + 4j of rank row g; of `up` (stored transposed),
 // the piece at rows 8g.. of ranks 2t, 2t+1 (+8).  What a 16-bit operand loses
 // of x and v goes into further parts, one instruction each (two TF32 parts on
-// both sides for fp32 weights), fp16 parts scaled by a power of two.
+// both sides for fp32 weights, heads and tails added up apart, as an instruction
+// cuts its sums off at their size), fp16 parts scaled by a power of two.
 //
 // A block sorts the tokens by adapter first (group_kernel, 7 us for 2049
 // tokens); tokens without one are copied.  x and out bound it at best; at
@@ -557,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                   const uint32_t(&f)[4] = ax[j][h][p];
                   if (K::f32) {
                     const float b0 = __uint_as_float(b[2 * h]), b1 = __uint_as_float(b[2 * h + 1]);
-                    mma::mma16<K::mode>(acc[0], f[0], f[1], f[2], f[3], mma::tf32_head(b0), mma::tf32_head(b1));
+                    mma::mma16<K::mode>(acc[p], f[0], f[1], f[2], f[3], mma::tf32_head(b0), mma::tf32_head(b1));
                     if (p == 0) mma::mma16<K::mode>(acc[1], f[0], f[1], f[2], f[3], mma::tf32_tail(b0), mma::tf32_tail(b1));
                   } else {
                     mma::mma16<K::mode>(acc[h], f[0], f[1], f[2], f[3], b[2 * h], b[2 * h + 1]);
@@ -618,6 +619,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int e = 0; e < K::epc; ++e)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[e][i] = 0.f;
+    float tails[K::f32 ? K::epc : 1][4] = {};
     // this lane's results: the 2 epc rows from mu + 2t epc on of tokens g and g + 8
     const int row0 = mu + 2 * t * K::epc;
     float base[2][2 * K::epc];
@@ -663,10 +665,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         };
         if (K::f32) {
           const float b0 = __uint_as_float(word(0)), b1 = __uint_as_float(word(1));
-#pragma unroll
-          for (int p = 0; p < K::pv; ++p)
-            mma::mma16<K::mode>(acc[e], f[p][0], f[p][1], f[p][2], f[p][3], mma::tf32_head(b0), mma::tf32_head(b1));
-          mma::mma16<K::mode>(acc[e], f[0][0], f[0][1], f[0][2], f[0][3], mma::tf32_tail(b0), mma::tf32_tail(b1));
+          float(&low)[4] = tails[e % (K::f32 ? K::epc : 1)];
+          mma::mma16<K::mode>(acc[e], f[0][0], f[0][1], f[0][2], f[0][3], mma::tf32_head(b0), mma::tf32_head(b1));
+          mma::mma16<K::mode>(low, f[K::pv - 1][0], f[K::pv - 1][1], f[K::pv - 1][2], f[K::pv - 1][3], mma::tf32_head(b0),
+                              mma::tf32_head(b1));
+          mma::mma16<K::mode>(low, f[0][0], f[0][1], f[0][2], f[0][3], mma::tf32_tail(b0), mma::tf32_tail(b1));
         } else {
           const uint32_t sel = e % 2 ? 0x7632 : 0x5410;
           const uint32_t b0 = __byte_perm(word(0), word(1), sel), b1 = __byte_perm(word(R - 2), word(R - 1), sel);
@@ -680,8 +683,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int tok = h ? token_g8 : token_g;
       T *p = static_cast<T *>(a.out.ptr) + row0 * a.out.stride[0] + tok * a.out.stride[1];
 #pragma unroll
-      for (int r = 0; r < 2 * K::epc; ++r, p += a.out.stride[0])
-        if (tok >= 0 && row0 + r < m1) *p = from_f32<T>(fmaf(acc[r % K::epc][2 * h + r / K::epc], vs[h], base[h][r]));
+      for (int r = 0; r < 2 * K::epc; ++r, p += a.out.stride[0]) {
+        float sum = acc[r % K::epc][2 * h + r / K::epc];
+        if (K::f32) sum += tails[r % (K::f32 ? K::epc : 1)][2 * h + r / K::epc];
+        if (tok >= 0 && row0 + r < m1) *p = from_f32<T>(fmaf(sum, vs[h], base[h][r]));
+      }
     }
   }
 }

@@ -659,11 +659,14 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
           };
           float acc[4] = {};
 #pragma unroll
-          for (int k = 0; k < PN; ++k) {
-            if (C::f32) {
+          for (int kt = 0; kt < (C::f32 ? 2 * PN : PN); ++kt) {
+            const int k = C::f32 ? kt % PN : kt;
+            if (C::f32) {  // tails first: the instruction cuts its sums off, small ones lose less
               const float v0 = __uint_as_float(word(2 * k)), v1 = __uint_as_float(word(2 * k + 1));
-              mma16<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], tf32_head(v0), tf32_head(v1));
-              mma16<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], tf32_tail(v0), tf32_tail(v1));
+              if (kt < PN)
+                mma16<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], tf32_tail(v0), tf32_tail(v1));
+              else
+                mma16<MODE>(acc, pa[k][0], pa[k][1], pa[k][2], pa[k][3], tf32_head(v0), tf32_head(v1));
             } else {
               const uint32_t sel = e % 2 ? 0x7632 : 0x5410;
               constexpr int two = C::f32 ? 0 : 4;

@@ -31,11 +31,14 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The TF32 head of x: its upper 11 significant bits; x - head is exact.
-__device__ __forceinline__ uint32_t tf32_head(float x) { return __float_as_uint(x) & 0xffffe000u; }
-__device__ __forceinline__ uint32_t tf32_tail(float x) {
-  return __float_as_uint(x - __uint_as_float(__float_as_uint(x) & 0xffffe000u));
-}
+// The TF32 head of x: x rounded to 11 significant bits; x - head is exact.  The
+// instruction cuts the tail to 11 bits too, which loses a unit of x's last place
+// at most.  With a head cut off in place of a rounded one the tail loses up to
+// three units, always towards zero: that put results off by 5e-7 (attention) and
+// 1.3e-6 (adapters) of their size, one way, where fp32 sums are off by 2e-7 and
+// 4e-7 either way.  A NaN that the addition carries over stays one in the tail.
+__device__ __forceinline__ uint32_t tf32_head(float x) { return (__float_as_uint(x) + 0x1000u) & 0xffffe000u; }
+__device__ __forceinline__ uint32_t tf32_tail(float x) { return __float_as_uint(x - __uint_as_float(tf32_head(x))); }
 
 // The power of two that brings a row of largest value `top` to below 2^15 for a
 // split into two fp16 parts: no part overflows, and values down to 2^-40 of the

@@ -87,3 +87,47 @@ def test_adapters_with_an_outlier_that_meets_zeros(cuda, kind, stored, tokens, w
     got = s.apply(x.cuda(), ids.cuda()).cpu().double()
     want, tol = ref.adapters(x, ids, [down], [up], [1.0], None, kind)
     assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+# fp32 operands are split into two parts of 11 bits.  Rounding a part errs either way; cutting it off takes 0.9 units of
+# 2^-23 of each operand's binade on average (0.6 of its size), always towards zero: 7e-8 an operand, and a product of
+# two such tails that is left out another 1e-7.  Below, every sum has one product, so that nothing but the split and
+# three or four roundings of 2^-24, which average out over 4096 results, and the constants' own (1.3e-8) is in the mean.
+
+def spread(gen, *shape):
+    """Numbers of either sign with mantissas spread evenly."""
+    sign = torch.randint(0, 2, shape, generator=gen).float() * 2 - 1
+    return sign * (1 + torch.rand(*shape, generator=gen)) * torch.randint(0, 4, shape, generator=gen).float().exp2()
+
+
+def mean_off(got, want):
+    return ((got - want) / want).mean().abs()
+
+
+def test_scores_and_values_of_fp32_are_split_without_a_bias(cuda):
+    gen = torch.Generator().manual_seed(43)
+    seqs, heads, d = 64, 64, 64
+    q, k = torch.zeros(seqs, heads, d), torch.zeros(seqs, heads, 16, d)
+    at = torch.arange(heads)
+    q[:, at, at] = spread(gen, seqs, heads)
+    k[:, at, 0, at] = spread(gen, seqs, heads)
+    v = spread(gen, seqs, heads, 16, d)
+    out, lse, _ = attention(q, k, v, [1] * seqs, 16)
+    z = q[:, at, at].double() * k[:, at, 0, at].double() / 8
+    assert mean_off(lse, z) <= 2.0 ** -24
+    assert mean_off(out, v[:, :, 0].double()) <= 2.0 ** -25
+
+
+def test_adapters_of_fp32_are_split_without_a_bias(cuda):
+    gen = torch.Generator().manual_seed(44)
+    k, m, tokens = 64, 64, 512
+    down, x = torch.zeros(1, k), torch.zeros(k, tokens)
+    x[3] = spread(gen, tokens)
+    sets = [(spread(gen, 1), spread(gen, m, 1)) for _ in range(8)]
+    want, got = [], []
+    for w, up in sets:
+        down[0, 3] = w
+        s = sc.LowRankAdapters([down.cuda()], [up.cuda()], [1.0])
+        got.append(s.apply(x.cuda(), torch.zeros(tokens, dtype=torch.int32, device=cuda)).cpu().double())
+        want.append(up.double() * (w.double() * x[3].double()))
+    assert mean_off(torch.stack(got), torch.stack(want)) <= 2.0 ** -24
