@@ -367,6 +367,16 @@ __device__ __forceinline__ void split2(float x0, float x1, float y0, float y1, u
   }
 }
 
+// A sum of products in plain fp32: what stands in for a result of split operands that is not finite, as their parts make
+// NaN of an infinity.  Out of line: hardly any call takes it.
+template <class X, class W>
+__device__ __noinline__ float plain_dot(const X *x, int64_t x_step, const W *w, int64_t w_step, int n) {
+  float sum = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) sum += to_f32(x[i * x_step]) * to_f32(w[i * w_step]);
+  return sum;
+}
+
 template <class T, class W>
 __global__ void __launch_bounds__(kThreads, 2)
     tile_kernel(const __grid_constant__ SetView s, const __grid_constant__ sc_adapters_args a, const Sorted sorted) {
@@ -579,7 +589,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (r64 + r < rank) {
           float sum = 0.f;
           for (int w = 0; w < live; ++w) sum += part[w * kTile * 64 + i];
-          v_part[i / 64 * v_row + r64 + r] += sum;
+          sum += v_part[i / 64 * v_row + r64 + r];
+          if (k + kChunk >= k1 && !isfinite(sum) && i / 64 < n)
+            sum = plain_dot(static_cast<const T *>(a.x.ptr) + k0 * a.x.stride[0] + s_tokens[i / 64] * a.x.stride[1], a.x.stride[0],
+                            down + (r64 + r) * s.in_row + k0, 1, k1 - k0);
+          v_part[i / 64 * v_row + r64 + r] = sum;
         }
       }
       __syncthreads();
@@ -678,6 +692,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
     }
+    uint32_t bad = 0;  // results that are not finite, and not written yet
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int tok = h ? token_g8 : token_g;
@@ -686,8 +701,21 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int r = 0; r < 2 * K::epc; ++r, p += a.out.stride[0]) {
         float sum = acc[r % K::epc][2 * h + r / K::epc];
         if (K::f32) sum += tails[r % (K::f32 ? K::epc : 1)][2 * h + r / K::epc];
-        if (tok >= 0 && row0 + r < m1) *p = from_f32<T>(fmaf(sum, vs[h], base[h][r]));
+        const float y = fmaf(sum, vs[h], base[h][r]);
+        if (tok >= 0 && row0 + r < m1) {
+          if (isfinite(y))
+            *p = from_f32<T>(y);
+          else
+            bad |= 1u << (2 * K::epc * h + r);
+        }
       }
+    }
+    for (; bad; bad &= bad - 1) {
+      const int i = __ffs(bad) - 1, h = i / (2 * K::epc);
+      const int64_t m = row0 + i % (2 * K::epc), tok = h ? token_g8 : token_g;
+      float y = plain_dot(v + (g + 8 * h) * v_row, 1, up + m, s.out_row, rank);
+      if (a.base.ptr) y += to_f32(static_cast<const T *>(a.base.ptr)[m * a.base.stride[0] + tok * a.base.stride[1]]);
+      static_cast<T *>(a.out.ptr)[m * a.out.stride[0] + tok * a.out.stride[1]] = from_f32<T>(y);
     }
   }
 }
