@@ -377,7 +377,7 @@ void sc_attn_free(sc_attn *p);
 typedef struct sc_attn_args {
   int64_t seqs;
   int64_t type;               /* SC_TYPE_* of q and out */
-  sc_rows q, out;             /* (seqs, q_heads, head_dim) */
+  sc_rows q, out;             /* (seqs, q_heads, head_dim); out does not overlap q */
   float *lse;                 /* [seqs x q_heads] log of the softmax sums, or NULL */
   const int32_t *page_table;  /* [seqs x table_cols], row stride table_stride */
   int64_t table_cols, table_stride;

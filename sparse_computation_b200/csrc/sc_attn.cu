@@ -16,8 +16,9 @@ struct sc_attn {
   int qtiles = 0, q_rows = 0, sms = 0;
   uint32_t page_mul = 0, page_shift = 0;
   Variant same, other;  // q of the cache's type; q of another type
-  DeviceBlock mem;      // its own workspace, if any: status | 1 KB of zeros | arrivals | pieces | records
+  DeviceBlock mem;      // its own workspace, if any: status | 1 KB of zeros | arrivals | doubtful rows | pieces | records
   int *status = nullptr, *arrivals = nullptr;
+  uint32_t *doubtful = nullptr;
   float *heads = nullptr, *records = nullptr;
 };
 
@@ -25,7 +26,7 @@ namespace {
 
 // A plan without its workspace, and the layout of that in 4-byte words.
 struct Layout {
-  size_t words, heads, total;  // status, zeros and arrivals; pieces; all
+  size_t segments, words, heads, total;  // arrivals; status, zeros, arrivals and doubtful rows; pieces; all
 };
 
 std::unique_ptr<sc_attn> set_up(const sc_kv_cache *cache, int64_t q_heads, int64_t max_seqs, double scale, int64_t window,
@@ -75,7 +76,8 @@ std::unique_ptr<sc_attn> set_up(const sc_kv_cache *cache, int64_t q_heads, int64
                               : variant_for<kBF16Wide>(pool.head_dim, p->q_rows, limit);
   }
   const size_t piece = (size_t)p->same.piece;
-  layout.words = 64 + 256 + ((size_t)segments + 63) / 64 * 64;
+  layout.segments = ((size_t)segments + 63) / 64 * 64;
+  layout.words = 64 + 256 + 2 * layout.segments;
   layout.heads = (size_t)p->sms * std::max(p->same.warps, p->other.warps) * piece;
   layout.total = layout.words + layout.heads + (size_t)p->sms * 2 * piece;
   return p;
@@ -85,6 +87,7 @@ void give_workspace(sc_attn &p, void *at, const Layout &layout) {
   clear_words(at, layout.words * 4);
   p.status = static_cast<int *>(at);
   p.arrivals = p.status + 64 + 256;
+  p.doubtful = reinterpret_cast<uint32_t *>(p.arrivals + layout.segments);
   p.heads = reinterpret_cast<float *>(p.status + layout.words);
   p.records = p.heads + layout.heads;
 }
@@ -158,7 +161,7 @@ int sc_attn_decode(sc_attn *p, const sc_attn_args *a, void *stream) {
            p->page_mul, p->page_shift, (uint32_t)(p->pool.k_stride[0] / unit), (uint32_t)(p->pool.k_stride[2] / unit),
            (uint32_t)(p->pool.v_stride[0] / unit), (uint32_t)(p->pool.v_stride[2] / unit),
            (float)(p->scale * 1.4426950408889634), p->window, p->status,
-           reinterpret_cast<const uint8_t *>(p->status + 64), p->arrivals, p->heads, p->records};
+           reinterpret_cast<const uint8_t *>(p->status + 64), p->arrivals, p->doubtful, p->heads, p->records};
   // the most steps that these lengths can have; the true number is known on the device only
   int64_t keys = std::min<int64_t>(a->table_cols, INT32_MAX / p->pool.page_size) * p->pool.page_size;
   if (p->window) keys = std::min(keys, p->window + 15);

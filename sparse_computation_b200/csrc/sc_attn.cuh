@@ -73,6 +73,7 @@ struct Params {
   int *status;
   const uint8_t *zeros;  // 1 KB
   int *arrivals;   // [seqs * kv_heads * qtiles], zero between calls
+  uint32_t *doubtful;  // as many: rows (bits) of a query tile whose results are not finite, and the block (+ 1) that wrote them
   float *heads;    // [blocks][warps] pieces whose warp went on after them
   float *records;  // [blocks][2]
 };
@@ -158,8 +159,8 @@ __device__ __forceinline__ float4 ld_relaxed4(const float *p) {
   return v;
 }
 
-// Four neighbouring outputs.  Out of line: it is not worth a copy at each of its uses.
-static __device__ __noinline__ void store4(void *ptr, int type, int64_t i, int64_t stride, float4 y) {
+// Four neighbouring outputs; whether they are finite.  Out of line: it is not worth a copy at each of its uses.
+static __device__ __noinline__ bool store4(void *ptr, int type, int64_t i, int64_t stride, float4 y) {
   const float v[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -170,6 +171,7 @@ static __device__ __noinline__ void store4(void *ptr, int type, int64_t i, int64
     else
       static_cast<__nv_bfloat16 *>(ptr)[i + e * stride] = __float2bfloat16_rn(v[e]);
   }
+  return fabsf(y.x) + fabsf(y.y) + fabsf(y.z) + fabsf(y.w) < INFINITY;
 }
 
 // Keys [first, len) of a sequence; steps start at `start`, first rounded down
@@ -199,6 +201,13 @@ __device__ __forceinline__ int page_of(const Params &p, int key) {
 
 __device__ __forceinline__ float lse_of(float ref, float sum) { return (ref + log2f(sum)) * 0.69314718055994531f; }
 
+// Element i of an array of a type known at run time.
+__device__ __forceinline__ float element(const void *p, int type, int64_t i) {
+  return type == SC_TYPE_F32   ? static_cast<const float *>(p)[i]
+         : type == SC_TYPE_F16 ? __half2float(static_cast<const __half *>(p)[i])
+                               : __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+
 // A boundary between two blocks' runs: the place that an equal cut gives,
 // moved to an end of its segment when that is near, which saves a join, or
 // when no keys are left there.
@@ -220,12 +229,17 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
   __shared__ Cut s_cut[2];
   // pieces: sequence (-1: none), segment of it, and whether that began before (1) or only ends after (2) this run
   __shared__ int s_seq[2 * kMaxWarps], s_unit[2 * kMaxWarps], s_open[2 * kMaxWarps];
-  __shared__ int s_last;
+  __shared__ int s_last, s_doubt;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   const int W = blockDim.x / 32, D = FULL ? DP : (int)p.pool.head_dim;
   const int seqs = (int)p.a.seqs;
   const int units = (int)p.pool.kv_heads * p.qtiles;  // segments of a sequence
 
+  // A result that is not finite: its row is computed again at the end.
+  auto doubt = [&](int seq, int unit, int row) {
+    atomicOr(p.doubtful + (int64_t)seq * units + unit, (blockIdx.x + 1) << kQT | 1u << row);
+    s_doubt = 1;
+  };
   auto work = [&] {
   // ---- this block's run: a scan over the sequences, blockDim of them at a time
   auto places_of = [&](int s) {  // of one of its segments
@@ -248,6 +262,7 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
   more = __reduce_add_sync(~0u, more);
   if (lane == 0) s_more[warp] = more;
   if (tid < 2 * W) s_seq[tid] = -1;
+  if (tid == 0) s_doubt = 0;
   __syncthreads();
   auto sum_of = [&](const int *v, int below) {  // of the first `below` warps' sums
     return __reduce_add_sync(~0u, lane < below ? v[lane] : 0);
@@ -527,15 +542,14 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
     __syncwarp();
   };
 
-  float m = -INFINITY, l = 0.f;
   constexpr int ON = C::VJ * C::epc;
-  float o[ON][2];
-#pragma unroll
-  for (int i = 0; i < ON; ++i) o[i][0] = o[i][1] = 0.f;
 #pragma unroll 1
   for (;;) {
     open_portion();
     if (at >= we) break;
+    float m = -INFINITY, l = 0.f, o[ON][2];
+#pragma unroll
+    for (int i = 0; i < ON; ++i) o[i][0] = o[i][1] = 0.f;
     copy_q();
     open_window(page_of(p, key));
     place();
@@ -713,7 +727,6 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
             y.w += __shfl_xor_sync(~0u, y.w, 16);
           }
           if (d < DP && g < rows) *reinterpret_cast<float4 *>(to + g * C::o_row + d) = y;
-          o[b][k] = o[b + 1][k] = o[b + 2][k] = o[b + 3][k] = 0.f;
         }
     if (t == 0 && g < rows) {
       to[kQT * C::o_row + g] = m;
@@ -726,9 +739,10 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
         const int r = i / (D / 4), d = i % (D / 4) * 4;
         const float sum = to[kQT * C::o_row + kQT + r], scale = sum == 0.f ? 0.f : 1.f / sum;
         const float4 y = *reinterpret_cast<const float4 *>(to + r * C::o_row + d);
-        store4(p.a.out.ptr, (int)p.a.type,
-               seq * p.a.out.stride[0] + (head0 + r) * p.a.out.stride[1] + d * p.a.out.stride[2],
-               p.a.out.stride[2], make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale));
+        if (!store4(p.a.out.ptr, (int)p.a.type,
+                    seq * p.a.out.stride[0] + (head0 + r) * p.a.out.stride[1] + d * p.a.out.stride[2], p.a.out.stride[2],
+                    make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale)))
+          doubt(seq, unit, r);
       }
       if (p.a.lse && t == 0 && g < rows)
         p.a.lse[(int64_t)seq * p.q_heads + head0 + g] = lse_of(m == -INFINITY ? 0.f : m, l);
@@ -736,8 +750,6 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
       const int i = 2 * warp + tail;
       s_seq[i] = seq, s_unit[i] = unit, s_open[i] = open;
     }
-    m = -INFINITY;
-    l = 0.f;
   }
 
   __syncthreads();
@@ -859,9 +871,10 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
         if (record) {
           if (d < DP) *reinterpret_cast<float4 *>(rec + r * C::o_row + d) = y[k];
         } else if (d < D) {
-          store4(p.a.out.ptr, (int)p.a.type,
-                 at_seq * p.a.out.stride[0] + head * p.a.out.stride[1] + d * p.a.out.stride[2], p.a.out.stride[2],
-                 make_float4(y[k].x * scale, y[k].y * scale, y[k].z * scale, y[k].w * scale));
+          if (!store4(p.a.out.ptr, (int)p.a.type,
+                      at_seq * p.a.out.stride[0] + head * p.a.out.stride[1] + d * p.a.out.stride[2], p.a.out.stride[2],
+                      make_float4(y[k].x * scale, y[k].y * scale, y[k].z * scale, y[k].w * scale)))
+            doubt(at_seq, at_unit, r);
         }
       }
       if (lane == 0) {
@@ -876,6 +889,62 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
   }
   };
   work();
+
+  // Doubtful rows that this block wrote, once more by plain fp32 products, a key after the other, a warp together.  An
+  // infinity among keys, values or queries makes NaN of split operands (the parts of one side meet it with either sign,
+  // or zero) where the formula has a weight of zero or an infinite result.  It stands here, and takes few registers
+  // rather than little time (a microsecond a key), as a call from above made the loop over the keys spill: 3 to 5 % of
+  // fp32 queries over fp16.
+  __syncthreads();
+  if (s_doubt)
+#pragma unroll 1
+    for (int i = warp; i < (min(s_cut[1].seq, seqs - 1) - s_cut[0].seq + 1) * units; i += W) {
+      const int s = s_cut[0].seq + i / units, unit = i % units, h = unit / p.qtiles, type = (int)p.pool.type;
+      uint32_t *word = p.doubtful + (int64_t)s * units + unit;
+      uint32_t rows = __shfl_sync(~0u, *static_cast<volatile uint32_t *>(word), 0);
+      if (rows >> kQT != blockIdx.x + 1) continue;
+      __syncwarp();
+      if (lane == 0) *word = 0;
+      const Span sp = span_of<C::keys>(p, s);
+#pragma unroll 1
+      for (rows &= (1u << kQT) - 1; rows; rows &= rows - 1) {
+        const int head = h * p.group + (unit - h * p.qtiles) * kQT + __ffs(rows) - 1;
+        const int64_t q0 = s * p.a.q.stride[0] + head * p.a.q.stride[1];
+#pragma unroll 1
+        for (int d0 = 0; d0 < D; d0 += 32) {
+          const int mine = min(d0 + lane, D - 1);
+          float top = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll 1
+          for (int key = sp.first; key < sp.len && !isnan(sum); ++key) {  // a NaN there is one in every result
+            const int page = page_of(p, key), e = p.a.page_table[s * p.a.table_stride + page];
+            if (e < 0 || e >= p.pool.num_pages) continue;
+            const int64_t slot = key - page * (int)p.pool.page_size;
+            const int64_t at_k = e * p.pool.k_stride[0] + h * p.pool.k_stride[1] + slot * p.pool.k_stride[2];
+            float z = 0.f;
+#pragma unroll 1
+            for (int d = lane; d < D; d += 32)
+              z += element(p.a.q.ptr, (int)p.a.type, q0 + d * p.a.q.stride[2]) * element(p.pool.k, type, at_k + d);
+#pragma unroll
+            for (int d = 16; d; d >>= 1) z += __shfl_xor_sync(~0u, z, d);
+            z *= p.scale_log2;
+            const float m = fmaxf(top, z), ref = m == -INFINITY ? 0.f : m, shrink = ex2(top - ref), weight = ex2(z - ref);
+            top = m;
+            sum = sum * shrink + weight;
+            o = o * shrink + weight * element(p.pool.v, type, e * p.pool.v_stride[0] + h * p.pool.v_stride[1] +
+                                                                  slot * p.pool.v_stride[2] + mine);
+          }
+          const float y = sum == 0.f ? 0.f : o / sum;
+          const int64_t to = s * p.a.out.stride[0] + head * p.a.out.stride[1] + mine * p.a.out.stride[2];
+          if (p.a.type == SC_TYPE_F32)
+            static_cast<float *>(p.a.out.ptr)[to] = y;
+          else if (p.a.type == SC_TYPE_F16)
+            static_cast<__half *>(p.a.out.ptr)[to] = __float2half_rn(y);
+          else
+            static_cast<__nv_bfloat16 *>(p.a.out.ptr)[to] = __float2bfloat16_rn(y);
+          if (p.a.lse && lane == 0) p.a.lse[(int64_t)s * p.q_heads + head] = lse_of(top == -INFINITY ? 0.f : top, sum);
+        }
+      }
+    }
 
   // sequences without keys; the blocks share them
 #pragma unroll 1

@@ -278,8 +278,8 @@ class DecodeAttention(_Handle):
     def attend(self, q, page_table, seq_lens, out=None, return_lse: bool = False, stream=None):
         """out[s] = softmax(scale q[s] k^T) v over the ``seq_lens[s]`` first
         keys of sequence s, whose pages row s of ``page_table`` lists.  q and
-        out: [seqs, q_heads, head_dim] of one type.  A sequence of length 0
-        gives zeros (lse -inf).  Returns out, or (out, lse [seqs, q_heads])."""
+        out: [seqs, q_heads, head_dim] of one type, apart in memory.  A sequence
+        of length 0 gives zeros (lse -inf).  Returns out, or (out, lse [seqs, q_heads])."""
         dev, dtype = self.device, q.dtype
         if stream is not None:
             return _on(stream, dev, (q, page_table, seq_lens, out),
