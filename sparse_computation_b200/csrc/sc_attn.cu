@@ -12,7 +12,7 @@ struct sc_attn {
   sc_kv_pool pool;
   int device = 0;
   int64_t q_heads = 0, max_seqs = 0, window = 0;
-  float scale = 0.f;
+  float scale_log2 = 0.f;
   int qtiles = 0, q_rows = 0, sms = 0;
   uint32_t page_mul = 0, page_shift = 0;
   Variant same, other;  // q of the cache's type; q of another type
@@ -35,7 +35,8 @@ std::unique_ptr<sc_attn> set_up(const sc_kv_cache *cache, int64_t q_heads, int64
   require(q_heads > 0 && q_heads % pool.kv_heads == 0 && q_heads <= 65535, SC_ERR_ARG,
           "q_heads must be a positive multiple of kv_heads");
   require(max_seqs > 0 && max_seqs <= (1 << 20), SC_ERR_ARG, "max_seqs must be 1 to 2^20");
-  require(std::isfinite(scale) && scale >= 0, SC_ERR_ARG, "scale must be positive and finite");
+  require(std::isfinite((float)(scale * 1.4426950408889634)) && scale >= 0, SC_ERR_ARG,
+          "scale must be positive and finite, in fp32 too");
   require(window >= 0, SC_ERR_ARG, "negative window");
   std::unique_ptr<sc_attn> p(new sc_attn);
   p->pool = pool;
@@ -43,7 +44,7 @@ std::unique_ptr<sc_attn> set_up(const sc_kv_cache *cache, int64_t q_heads, int64
   p->q_heads = q_heads;
   p->max_seqs = max_seqs;
   p->window = std::min<int64_t>(window, INT32_MAX);
-  p->scale = (float)(scale > 0 ? scale : 1.0 / std::sqrt((double)pool.head_dim));
+  p->scale_log2 = (float)((scale > 0 ? scale : 1.0 / std::sqrt((double)pool.head_dim)) * 1.4426950408889634);
   p->qtiles = (int)((q_heads / pool.kv_heads + kQT - 1) / kQT);
   const int64_t segments = max_seqs * pool.kv_heads * p->qtiles;
   // a run of one block is counted in 32 bits
@@ -160,7 +161,7 @@ int sc_attn_decode(sc_attn *p, const sc_attn_args *a, void *stream) {
   Params k{*a, p->pool, (int)p->q_heads, (int)(p->q_heads / p->pool.kv_heads), p->qtiles, p->q_rows, v.warps, q_vec,
            p->page_mul, p->page_shift, (uint32_t)(p->pool.k_stride[0] / unit), (uint32_t)(p->pool.k_stride[2] / unit),
            (uint32_t)(p->pool.v_stride[0] / unit), (uint32_t)(p->pool.v_stride[2] / unit),
-           (float)(p->scale * 1.4426950408889634), p->window, p->status,
+           p->scale_log2, p->window, p->status,
            reinterpret_cast<const uint8_t *>(p->status + 64), p->arrivals, p->doubtful, p->heads, p->records};
   // the most steps that these lengths can have; the true number is known on the device only
   int64_t keys = std::min<int64_t>(a->table_cols, INT32_MAX / p->pool.page_size) * p->pool.page_size;

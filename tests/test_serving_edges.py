@@ -35,3 +35,12 @@ def test_refusals_of_weights_without_two_dimensions(cuda):
         with pytest.raises(sc.ScError) as e:
             sc.LowRankAdapters([down], [up], [1.0])
         assert e.value.code == sc.SC_ERR_ARG
+
+
+def test_a_scale_beyond_fp32_is_refused(cuda):
+    cache = sc.PagedKVCache.allocate(4, 16, 2, 64)
+    for scale in (1e39, 3e38, 1e308):  # 3e38 / ln 2 is beyond fp32 too
+        with pytest.raises(sc.ScError) as e:
+            sc.DecodeAttention(cache, 4, 4, scale=scale)
+        assert e.value.code == sc.SC_ERR_ARG
+    sc.DecodeAttention(cache, 4, 4, scale=1e38)
