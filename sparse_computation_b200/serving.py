@@ -72,17 +72,17 @@ def _table(t, device: int) -> tuple:
     return t.data_ptr(), n, c, s
 
 
-def _on(stream, device: int, given, call):
-    """call() with ``stream`` current, so that outputs and scratch come from that stream's memory: a block that is free
+def _on(stream, device: int, given, call, *args):
+    """call(*args) with ``stream`` current, so that outputs and scratch come from that stream's memory: a block that is free
     on the stream that is current here may still have its last kernel ahead of it, and ``stream`` does not wait for
     that.  The tensors of the call are kept from reuse until both streams are done with them."""
     if stream.device.index != device:
         _fail(f"the stream is on {stream.device}, the call on cuda:{device}")
     here = torch.cuda.current_stream(device)
     if stream == here:
-        return call()
+        return call(*args)
     with torch.cuda.stream(stream):
-        got = call()
+        got = call(*args)
     for t in given:
         if t is not None:
             t.record_stream(stream)
@@ -125,16 +125,12 @@ class _Handle:
         self._release = getattr(lib(), self._free)  # module globals may be gone when the interpreter ends
         self._call = getattr(lib(), self._run)
 
-    def _stream(self) -> int:
-        """The raw current stream, for a launch.  The handle's memory is kept from reuse until that stream is done with
-        it, however early the handle is dropped; once for each stream is enough, as the allocator looks when it is
-        freed."""
-        raw = _current(self.device)
-        if raw not in self._streams:
-            for t in self._kept:
-                t.record_stream(torch.cuda.current_stream(self.device))
-            self._streams.add(raw)
-        return raw
+    def _keep(self, raw: int) -> None:
+        """Keeps the handle's memory from reuse until the current stream, ``raw``, is done with it, however early the
+        handle is dropped.  Once for each stream is enough, as the allocator looks when the memory is freed."""
+        for t in self._kept:
+            t.record_stream(torch.cuda.current_stream(self.device))
+        self._streams.add(raw)
 
     def __del__(self):
         if self._h is not None:
@@ -205,7 +201,7 @@ class PagedKVCache(_Handle):
         if stream is not None:
             return _on(stream, dev, (k, v, positions, seq_ids, page_table, q, q_out,
                                      *((rope.cos, rope.sin) if rope is not None else ())),
-                       lambda: self.append(k, v, positions, page_table, seq_ids, rope, q, q_out))
+                       self.append, k, v, positions, page_table, seq_ids, rope, q, q_out)
         kind = _TYPES.get(dtype)
         if kind is None or k.dim() != 3:
             _fail("k must be a 3-D float32, float16 or bfloat16 tensor")
@@ -244,8 +240,11 @@ class PagedKVCache(_Handle):
             if n:
                 _fail("an empty page table")
             return q_out
+        s = _current(dev)
+        if s not in self._streams:
+            self._keep(s)
         bad = self._call(self._h, _APPEND.pack(n, heads, kind, *ka, *va, *qa, *oa, pos, ids, tab, seqs, cols, tstride,
-                                               *ra), self._stream())
+                                               *ra), s)
         if bad:
             _check(bad)
         return q_out
@@ -282,8 +281,7 @@ class DecodeAttention(_Handle):
         of length 0 gives zeros (lse -inf).  Returns out, or (out, lse [seqs, q_heads])."""
         dev, dtype = self.device, q.dtype
         if stream is not None:
-            return _on(stream, dev, (q, page_table, seq_lens, out),
-                       lambda: self.attend(q, page_table, seq_lens, out, return_lse))
+            return _on(stream, dev, (q, page_table, seq_lens, out), self.attend, q, page_table, seq_lens, out, return_lse)
         kind = _TYPES.get(dtype)
         if kind is None or q.dim() != 3:
             _fail("q must be a 3-D float32, float16 or bfloat16 tensor")
@@ -304,8 +302,11 @@ class DecodeAttention(_Handle):
         lens = _ints(seq_lens, "seq_lens", dev, n)
         lse = q.new_empty((n, self.q_heads), dtype=torch.float32) if return_lse else None
         if n:
+            s = _current(dev)
+            if s not in self._streams:
+                self._keep(s)
             bad = self._call(self._h, _ATTEND.pack(n, kind, *qa, *oa, lse.data_ptr() if return_lse else 0, tab, cols,
-                                                   tstride, lens), self._stream())
+                                                   tstride, lens), s)
             if bad:
                 _check(bad)
         return (out, lse) if return_lse else out
@@ -373,7 +374,7 @@ class LowRankAdapters(_Handle):
         negative for a token without an adapter.  out may be base."""
         dev, dtype = self.device, x.dtype
         if stream is not None:
-            return _on(stream, dev, (x, ids, base, out), lambda: self.apply(x, ids, base, out))
+            return _on(stream, dev, (x, ids, base, out), self.apply, x, ids, base, out)
         kind = _TYPES.get(dtype)
         if kind is None or x.dim() != 2:
             _fail("x must be a 2-D float32, float16 or bfloat16 tensor")
@@ -396,8 +397,11 @@ class LowRankAdapters(_Handle):
         if n:
             size = self._workspace(n)
             work = x.new_empty(size, dtype=torch.uint8) if size else None
+            s = _current(dev)
+            if s not in self._streams:
+                self._keep(s)
             bad = self._call(self._h, _ADAPT.pack(n, kind, *xa, *ba, *oa, idp, work.data_ptr() if size else 0, size),
-                             self._stream())
+                             s)
             if bad:
                 _check(bad)
         return out
