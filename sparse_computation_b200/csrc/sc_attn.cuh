@@ -515,7 +515,8 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
       up = f16_scale(top);
     }
-    c = p.scale_log2 * up;
+    // not zero: the -inf of a masked key stays one; scores of so small a factor are zero in any case
+    c = fmaxf(p.scale_log2 * up, 1.17549435e-38f);
 #pragma unroll 1
     for (int j = 0; j < C::KJ; ++j) {
       float x[C::epc];

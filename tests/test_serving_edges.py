@@ -44,3 +44,26 @@ def test_a_scale_beyond_fp32_is_refused(cuda):
             sc.DecodeAttention(cache, 4, 4, scale=scale)
         assert e.value.code == sc.SC_ERR_ARG
     sc.DecodeAttention(cache, 4, 4, scale=1e38)
+
+
+@pytest.mark.parametrize("kind,stored", [(F32, F32), (F32, BF16), (F32, F16), (BF16, BF16), (F16, F16), (BF16, F16)])
+@pytest.mark.parametrize("scale,size", [(1e-50, 1.0), (1e-9, 0.0), (1e-9, 2.0 ** -120), (1e-30, 1.0)])
+def test_scales_and_queries_near_zero_weigh_all_keys_alike(cuda, kind, stored, scale, size):
+    """A product of scale and query below fp32's smallest number is a score of zero, also beside keys that are masked."""
+    gen = torch.Generator().manual_seed(31)
+    lens, page, d = [21, 1, 0, 300], 16, 64
+    need = [-(-n // page) for n in lens]
+    table, at = torch.zeros(len(lens), max(need), dtype=torch.int32), 0
+    for i, c in enumerate(need):
+        table[i, :c] = torch.arange(at, at + c).int()
+        at += c
+    k, v = (torch.randn(at, 2, page, d, generator=gen).to(stored) for _ in range(2))
+    q = (torch.randn(len(lens), 4, d, generator=gen) * size).to(kind)
+    plan = sc.DecodeAttention(sc.PagedKVCache(k.cuda(), v.cuda()), 4, len(lens), scale=scale)
+    out, lse = plan.attend(q.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), return_lse=True)
+    plan.check()
+    w, wl, tol, ltol = ref.attend(q, k, v, table, lens, scale)
+    assert ((out.cpu().double() - w).abs() <= tol).all()
+    there = wl != -math.inf
+    assert torch.equal(lse.cpu() != -math.inf, there)
+    assert ((lse.cpu().double() - wl)[there].abs() <= ltol[there]).all()
