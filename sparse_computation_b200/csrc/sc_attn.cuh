@@ -891,61 +891,90 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
   };
   work();
 
-  // Doubtful rows that this block wrote, once more by plain fp32 products, a key after the other, a warp together.  An
-  // infinity among keys, values or queries makes NaN of split operands (the parts of one side meet it with either sign,
-  // or zero) where the formula has a weight of zero or an infinite result.  It stands here, and takes few registers
-  // rather than little time (a microsecond a key), as a call from above made the loop over the keys spill: 3 to 5 % of
-  // fp32 queries over fp16.
+  // Doubtful rows that this block wrote, once more by plain fp32 products.  An infinity among keys, values or queries
+  // makes NaN of split operands (the parts of one side meet it with either sign, or zero) where the formula has a weight
+  // of zero or an infinite result.  A warp takes a row, 32 keys at a time: a lane its key's score, then four dims of the sum.
+  // It takes 0.7 us a key (88 ms for a long document of 131071 keys with a NaN among its values), for memory that is
+  // broken as a rule.  It stands here and calls nothing: with a function call more, the loop over the keys spills (fp32
+  // queries over fp16 3 to 6 % slower).
   __syncthreads();
-  if (s_doubt)
+  if (s_doubt) {
+    const int words = (min(s_cut[1].seq, seqs - 1) - s_cut[0].seq + 1) * units;
+    uint32_t *const notes = p.doubtful + (int64_t)s_cut[0].seq * units;
 #pragma unroll 1
-    for (int i = warp; i < (min(s_cut[1].seq, seqs - 1) - s_cut[0].seq + 1) * units; i += W) {
-      const int s = s_cut[0].seq + i / units, unit = i % units, h = unit / p.qtiles, type = (int)p.pool.type;
-      uint32_t *word = p.doubtful + (int64_t)s * units + unit;
-      uint32_t rows = __shfl_sync(~0u, *static_cast<volatile uint32_t *>(word), 0);
-      if (rows >> kQT != blockIdx.x + 1) continue;
-      __syncwarp();
-      if (lane == 0) *word = 0;
+    for (int i = warp; i < words * p.q_rows; i += W) {
+      const int r = i % p.q_rows, s = s_cut[0].seq + i / p.q_rows / units, unit = i / p.q_rows % units, h = unit / p.qtiles;
+      const uint32_t note = *static_cast<volatile uint32_t *>(notes + i / p.q_rows);
+      if (note >> kQT != blockIdx.x + 1 || !(note >> r & 1)) continue;
       const Span sp = span_of<C::keys>(p, s);
+      const int head = h * p.group + (unit - h * p.qtiles) * kQT + r, type = (int)p.pool.type;
+      const int64_t q0 = s * p.a.q.stride[0] + head * p.a.q.stride[1];
 #pragma unroll 1
-      for (rows &= (1u << kQT) - 1; rows; rows &= rows - 1) {
-        const int head = h * p.group + (unit - h * p.qtiles) * kQT + __ffs(rows) - 1;
-        const int64_t q0 = s * p.a.q.stride[0] + head * p.a.q.stride[1];
+      for (int d0 = 0; d0 < D; d0 += 128) {
+        const int dim = d0 + lane;  // and 32, 64, 96 on
+        float top = -INFINITY, sum = 0.f, y[4] = {};
 #pragma unroll 1
-        for (int d0 = 0; d0 < D; d0 += 32) {
-          const int mine = min(d0 + lane, D - 1);
-          float top = -INFINITY, sum = 0.f, o = 0.f;
+        for (int key0 = sp.first; key0 < sp.len && !isnan(sum); key0 += 32) {  // a NaN there is one in every result
+          float z = -INFINITY;
+          int64_t at_v = -1;
+          if (key0 + lane < sp.len) {
+            const int page = page_of(p, key0 + lane), e = p.a.page_table[s * p.a.table_stride + page];
+            const int64_t slot = key0 + lane - page * (int)p.pool.page_size;
+            if (e >= 0 && e < p.pool.num_pages) {
+              at_v = e * p.pool.v_stride[0] + h * p.pool.v_stride[1] + slot * p.pool.v_stride[2];
+              const uint4 *k = reinterpret_cast<const uint4 *>(
+                  static_cast<const uint8_t *>(p.pool.k) +
+                  (e * p.pool.k_stride[0] + h * p.pool.k_stride[1] + slot * p.pool.k_stride[2]) * C::es);
+              z = 0.f;
 #pragma unroll 1
-          for (int key = sp.first; key < sp.len && !isnan(sum); ++key) {  // a NaN there is one in every result
-            const int page = page_of(p, key), e = p.a.page_table[s * p.a.table_stride + page];
-            if (e < 0 || e >= p.pool.num_pages) continue;
-            const int64_t slot = key - page * (int)p.pool.page_size;
-            const int64_t at_k = e * p.pool.k_stride[0] + h * p.pool.k_stride[1] + slot * p.pool.k_stride[2];
-            float z = 0.f;
-#pragma unroll 1
-            for (int d = lane; d < D; d += 32)
-              z += element(p.a.q.ptr, (int)p.a.type, q0 + d * p.a.q.stride[2]) * element(p.pool.k, type, at_k + d);
+              for (int d = 0; d < D; d += C::epc) {
+                const uint4 w = k[d / C::epc];
 #pragma unroll
-            for (int d = 16; d; d >>= 1) z += __shfl_xor_sync(~0u, z, d);
-            z *= p.scale_log2;
-            const float m = fmaxf(top, z), ref = m == -INFINITY ? 0.f : m, shrink = ex2(top - ref), weight = ex2(z - ref);
-            top = m;
-            sum = sum * shrink + weight;
-            o = o * shrink + weight * element(p.pool.v, type, e * p.pool.v_stride[0] + h * p.pool.v_stride[1] +
-                                                                  slot * p.pool.v_stride[2] + mine);
+                for (int c = 0; c < C::epc; ++c)
+                  z += element(p.a.q.ptr, (int)p.a.type, q0 + (d + c) * p.a.q.stride[2]) * element(&w, type, c);
+              }
+              z *= p.scale_log2;
+            }
           }
-          const float y = sum == 0.f ? 0.f : o / sum;
-          const int64_t to = s * p.a.out.stride[0] + head * p.a.out.stride[1] + mine * p.a.out.stride[2];
-          if (p.a.type == SC_TYPE_F32)
-            static_cast<float *>(p.a.out.ptr)[to] = y;
-          else if (p.a.type == SC_TYPE_F16)
-            static_cast<__half *>(p.a.out.ptr)[to] = __float2half_rn(y);
-          else
-            static_cast<__nv_bfloat16 *>(p.a.out.ptr)[to] = __float2bfloat16_rn(y);
-          if (p.a.lse && lane == 0) p.a.lse[(int64_t)s * p.q_heads + head] = lse_of(top == -INFINITY ? 0.f : top, sum);
+          float m = fmaxf(top, z);
+#pragma unroll
+          for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+          const float ref = m == -INFINITY ? 0.f : m, shrink = ex2(top - ref), weight = at_v < 0 ? 0.f : ex2(z - ref);
+          float all = weight;
+#pragma unroll
+          for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
+          top = m;
+          sum = sum * shrink + all;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) y[c] *= shrink;
+#pragma unroll 2
+          for (int k = 0; k < 32; ++k) {
+            const int64_t at = __shfl_sync(~0u, at_v, k);
+            const float w = __shfl_sync(~0u, weight, k);
+            if (at >= 0)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) y[c] += w * element(p.pool.v, type, at + min(dim + 32 * c, D - 1));
+          }
         }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float x = sum == 0.f ? 0.f : y[c] / sum;
+          const int64_t to = s * p.a.out.stride[0] + head * p.a.out.stride[1] + min(dim + 32 * c, D - 1) * p.a.out.stride[2];
+          if (p.a.type == SC_TYPE_F32)
+            static_cast<float *>(p.a.out.ptr)[to] = x;
+          else if (p.a.type == SC_TYPE_F16)
+            static_cast<__half *>(p.a.out.ptr)[to] = __float2half_rn(x);
+          else
+            static_cast<__nv_bfloat16 *>(p.a.out.ptr)[to] = __float2bfloat16_rn(x);
+        }
+        if (p.a.lse && lane == 0) p.a.lse[(int64_t)s * p.q_heads + head] = lse_of(top == -INFINITY ? 0.f : top, sum);
       }
     }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < words; i += blockDim.x)
+      if (notes[i] >> kQT == blockIdx.x + 1) notes[i] = 0;
+  }
 
   // sequences without keys; the blocks share them
 #pragma unroll 1
