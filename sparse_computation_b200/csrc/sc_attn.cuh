@@ -902,9 +902,10 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
     const int words = (min(s_cut[1].seq, seqs - 1) - s_cut[0].seq + 1) * units;
     uint32_t *const notes = p.doubtful + (int64_t)s_cut[0].seq * units;
 #pragma unroll 1
-    for (int i = warp; i < words * p.q_rows; i += W) {
-      const int r = i % p.q_rows, s = s_cut[0].seq + i / p.q_rows / units, unit = i / p.q_rows % units, h = unit / p.qtiles;
-      const uint32_t note = *static_cast<volatile uint32_t *>(notes + i / p.q_rows);
+    for (int64_t i = warp; i < (int64_t)words * p.q_rows; i += W) {
+      const int word = (int)(i / p.q_rows), r = (int)(i - (int64_t)word * p.q_rows);
+      const int s = s_cut[0].seq + word / units, unit = word % units, h = unit / p.qtiles;
+      const uint32_t note = *static_cast<volatile uint32_t *>(notes + word);
       if (note >> kQT != blockIdx.x + 1 || !(note >> r & 1)) continue;
       const Span sp = span_of<C::keys>(p, s);
       const int head = h * p.group + (unit - h * p.qtiles) * kQT + r, type = (int)p.pool.type;
