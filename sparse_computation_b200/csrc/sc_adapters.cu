@@ -62,9 +62,18 @@ __global__ void __launch_bounds__(256) pack_rows(const PackItem *list, W *dst) {
 // v = down x are added up through distributed shared memory, in block order;
 // then each block makes its part of the rows of up v.  One launch, no scratch
 // memory.  Bound by latency (a chain of ids, weights, two cluster barriers,
-// weights) and fp32 instructions; the tensor-core tiles below have twice the
-// fixed cost: 128 tokens of 100 adapters of 512 x 2048 in bf16 take 14.8 us
-// here, 28.6 there; 96 tokens of 40 adapters of 4096 x 4096 21.4 and 33.3.
+// weights) and fp32 instructions; the tensor-core tiles below cost more before
+// they start, and less for each further token of an adapter.  us here / there
+// for 1, 2, 4, 8, 16 and 64 tokens an adapter, 512 x 2048 of rank 16 in bf16:
+//   64 tokens  12.5/16.1   9.3/15.6 10.5/14.9 10.6/14.3 11.3/14.7 10.7/14.4
+//   128        15.8/22.9  12.2/17.1 13.8/16.1 14.5/15.8 15.8/15.3 15.5/14.5
+//   256        23.4/42.6  19.2/24.6 30.3/23.1 30.5/18.3 28.6/19.0 28.9/16.0
+// and 4096 x 4096 of ranks 16 to 64 in bf16:
+//   128        56.5/93.9  46.1/53.5 27.1/38.3 27.5/27.7 27.6/28.5 24.1/27.6
+//   256       105.9/171.6 70.8/96.5 61.1/91.7 54.1/46.7 45.5/35.5 45.5/35.9
+// How tokens spread over adapters is known on the device only, so the rule goes
+// by their number: up to 256, where a thread of a block looks at each token's
+// id.  From about 8 tokens an adapter and 200 tokens on the tiles would be faster.
 constexpr int kFewTokens = 256, kGroup = 4 /* a float4 of v */, kFewChunk = 512, kFewThreads = 256, kFewBlocks = 3;
 
 // Eight weights, as they lie.

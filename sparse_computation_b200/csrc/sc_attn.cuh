@@ -12,7 +12,8 @@
 // rows.  Rows that a group of heads leaves free carry what a single 16-bit or
 // TF32 operand loses: Q and P are split into parts that share one instruction
 // (head in rows 0-7, tail in rows 8-15), and the parts of the result are
-// added.  16-bit queries of the cache's type need no parts; fp32 queries over
+// added.  16-bit queries of the cache's type need no parts (P has two for them:
+// 16 bits or more, below the rounding of their results); fp32 queries over
 // fp16 two, over bf16 three: those fit one instruction for groups of up to
 // four (rows 0-3, 4-7, 8-11: kBF16Wide4) and take two for larger ones.  An fp32
 // cache is split too, into TF32 heads and tails: two instructions.
@@ -27,7 +28,7 @@
 // product with P.  At 8 KB a warp step and 12 warps a SM that is 48-96 KB in
 // flight, more than latency times bandwidth asks for.  A version with 16 warps
 // that went through cp.async and shared memory took 147 us at 131071 keys (8
-// kv heads of 128, bf16), a fifth of it in a slower join; this takes 92, 5.8
+// kv heads of 128, bf16), a fifth of it in a slower join; this takes 94, 5.7
 // TB/s.  Row addresses are computed where they are needed: handing them round
 // by shuffles cost a fifth of the loop's speed.
 //
@@ -45,7 +46,7 @@
 // What is left over the read: the scan, the first loads, and the two joins, 5
 // to 10 us in all, most of it fetching code that each block runs once (25
 // cycles an instruction while the memory is busy).  128 fp32 requests of 16 to
-// 1024 keys, 8 heads of 64: 39 us against 19 for the bytes; 32 requests of 100
+// 1024 keys, 8 heads of 64: 40 us against 19 for the bytes; 32 requests of 100
 // to 8192 keys, 32 / 8 heads of 128, fp32 queries over bf16: 63 against 39.
 #pragma once
 
@@ -101,9 +102,10 @@ struct Cfg {
   static constexpr int q_row = KJ * parts * 64;              // bytes of one query row in fragment order
   static constexpr int max_warps = DP > 128 ? 8 : kMaxWarps;  // by the registers of a step
   // Segments are laid end to end with this many places after each that hold no keys: they stand for what changing to
-  // another segment costs a warp (its query, its pages, its result) in steps.  us of 128 fp32 requests / of the ragged
-  // bf16 batch / of windows over fp16: 38.6 69.7 28.7 with 1, 39.9 65.5 26.4 with 2, 40.8 62.7 26.1 with 3, 42.1 61.9
-  // 26.9 with 4.
+  // another segment costs a warp (its query, its pages, its result) in steps.  us with 1 / 2 / 3 / 4, fp32 caches: 128
+  // requests of 16-1024 keys 40.0 41.2 41.9 43.8, 64 of 50-3000 50.6 51.3 51.4 52.5, 37 of 1-700 (4 kv heads of 128)
+  // 22.0 23.4 23.2 23.2; 16 bits: 32 of 100-8192 70.1 65.5 62.6 62.6, 48 of 1-2500 39.1 33.6 32.6 32.8, 61 windows of
+  // 1000 30.0 27.3 27.2 28.0, 100 windows of 500 22.2 22.3 22.5 22.6.
   static constexpr int change = f32 ? 1 : 3;
   // P (1 at most) as it is split into fp16 parts: two parts then keep weights down to 2^-38 of the largest, where fp16's
   // smallest value would cut those of e^-16 to a single bit.  Taken off again where a portion's result is written.
@@ -271,7 +273,8 @@ __global__ void __launch_bounds__(Cfg<MODE, DP>::max_warps * 32, 1) attend_kerne
   const int total = (chunk + sum_of(s_more, W)) * units;
   const int per = max((int)((total + gridDim.x - 1) / gridDim.x), p.min_run);
   // A join costs about what a block's eighth does, or half a step of every warp: with a quarter of either the smallest
-  // batch took 14 us instead of 11.4, with twice the eighth the ragged one 66.8 instead of 62.6.
+  // batch took 14.2 us instead of 11.8 and 48 requests of 1-2500 keys 34.6 instead of 32.5; with twice the eighth 32 of
+  // 100-8192 keys 66.8 instead of 62.6 and 64 fp32 ones of 50-3000 56.4 instead of 50.5 (61 windows 26.3, not 27.2).
   const int near = max(per / 8, min(per, W) / 2);
   const int nominal0 = per * blockIdx.x, nominal1 = nominal0 + per;
   if (nominal0 >= total) return;

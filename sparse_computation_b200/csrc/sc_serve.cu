@@ -296,8 +296,8 @@ __global__ void __launch_bounds__(128, 4) append_rows_kernel(const __grid_consta
 // turns it in shared memory and writes it along the dims, two to a thread, or
 // eight for prompts.  Bound by the chain of latencies (position, page entry,
 // rotation row, store) at decoding sizes: 128 tokens of 32 + 2 x 8 heads of 128,
-// fp32 into bf16, 5.3 us against 0.9 for their bytes; 4 tokens of 3 x 8 heads
-// of 64 2.0 us.
+// fp32 into bf16, 5.7 us against 0.9 for their bytes; 4 tokens of 3 x 8 heads
+// of 64 2.4 us.  2000 tokens of the former 36 us against 14.
 template <class T, class C>
 __global__ void __launch_bounds__(256) append_columns_kernel(const __grid_constant__ AppendParams p) {
   const sc_kv_append_args &a = p.a;
@@ -541,7 +541,9 @@ int sc_kv_append(sc_kv_cache *c, const sc_kv_append_args *a, void *stream) {
       p.tile_bits = 5;
       while (p.tile_bits > fewest && heads * (a->tokens >> p.tile_bits) < 4 * 148) --p.tile_bits;
       while (p.tile_bits > 2 && a->tokens <= 1 << (p.tile_bits - 1)) --p.tile_bits;
-      // eights have fewer instructions, pairs more threads: 2000 tokens 21.3 us against 23.8, 4 tokens 2.6 against 2.0
+      // Eights have fewer instructions, pairs more threads.  us in eights / in pairs for 4, 64, 256, 512 and 2000 fp32
+      // tokens into bf16, 32 + 2 x 8 heads of 128: 3.0/2.5 3.8/4.0 7.3/8.6 10.9/14.8 36.2/46.5; 3 x 8 heads of 64:
+      // 3.1/2.4 3.4/3.1 5.5/4.8 5.7/5.9 10.9/13.2.
       if (p.tile_bits < 5) p.eights = 0;
       const Divider pairs(D / 2);
       p.pairs_mul = pairs.mul, p.pairs_shift = pairs.shift;
