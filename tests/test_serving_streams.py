@@ -190,7 +190,7 @@ def test_a_dropped_handle_keeps_its_memory_until_its_streams_are_done(cuda, expl
 
     def use(call):
         with torch.cuda.stream(side):
-            torch.cuda._sleep(20_000_000)  # about 10 ms
+            torch.cuda._sleep(200_000_000)  # about 0.1 s
             if not explicit:
                 return call()
         return call(stream=side)
@@ -234,7 +234,7 @@ def test_outputs_on_another_stream_take_no_block_of_the_current_one(cuda):
         size = call().numel()  # and loads the kernels
         torch.cuda.synchronize()
         freed = torch.empty(size, device=cuda)
-        torch.cuda._sleep(20_000_000)  # about 10 ms
+        torch.cuda._sleep(200_000_000)  # about 0.1 s
         freed.add_(1)
         at = freed.data_ptr()
         del freed
