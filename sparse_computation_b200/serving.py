@@ -273,6 +273,7 @@ class DecodeAttention(_Handle):
         at = (self._work.data_ptr() + 255) // 256 * 256
         _check(lib().sc_attn_create_in(cache._h, q_heads, max_seqs, scale or 0.0, window, at, size.value, ctypes.byref(h)))
         self._own(h, self._work, cache.k, cache.v)
+        self._streams &= cache._streams  # the cache may come from another stream's memory
 
     def attend(self, q, page_table, seq_lens, out=None, return_lse: bool = False, stream=None):
         """out[s] = softmax(scale q[s] k^T) v over the ``seq_lens[s]`` first

@@ -17,6 +17,9 @@ class Stream:
     def __init__(self, raw):
         self.cuda_stream, self.device = raw, SimpleNamespace(index=-1)
 
+    def synchronize(self):
+        pass
+
 
 MAIN, SIDE = Stream(1), Stream(2)
 
@@ -130,6 +133,27 @@ def test_a_stream_of_another_device_is_refused(recorder, name):
     with pytest.raises(sc.ScError) as e:
         call(stream=other)
     assert e.value.code == sc.SC_ERR_ARG and not recorder.launched
+
+
+def test_a_plan_made_on_another_stream_than_its_cache(recorder, monkeypatch):
+    """The cache's memory is kept for the plan's stream too, although the plan's own workspace comes from there."""
+    def size(cache, heads, seqs, out):
+        out._obj.value = 64
+        return 0
+
+    fake = SimpleNamespace(sc_attn_workspace=size, sc_attn_create_in=lambda *a: 0, sc_attn_free=lambda h: None,
+                           sc_attn_decode=lambda h, args, stream: recorder.launched.append(stream))
+    monkeypatch.setattr(serving, "lib", lambda: fake)
+    pools = torch.zeros(2, 4, 2, 4, 8)
+    cache = handle(recorder, sc.PagedKVCache, pools, k=pools[0], v=pools[1], kv_heads=2, head_dim=8)
+    cache._h = None
+    q, table, lens = torch.zeros(3, 2, 8), torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    with torch.cuda.stream(SIDE):
+        plan = sc.DecodeAttention(cache, 2, 3)
+        plan.attend(q, table, lens)
+    assert recorder.launched == [SIDE.cuda_stream]
+    for t in pools:
+        assert (SIDE.cuda_stream, t.data_ptr()) in recorder.kept
 
 
 def test_scratch_sizes_of_two_threads_stay_apart(recorder, monkeypatch):
